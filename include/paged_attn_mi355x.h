@@ -351,6 +351,48 @@ int pa_rotary_embedding_neox(
     int64_t query_stride, int64_t key_stride, int dtype, void* stream);
 
 /*
+ * Rotary embedding in place on query and key, in either pair layout and with
+ * numbers of query and key heads of their own.  No counterpart in the
+ * reference, whose only rotation is rotary_embedding_neox.
+ *
+ *   positions      [num_tokens] int64.  Negative: the token's rows are left as
+ *                  they are (padding).  >= max_position: what would be rotated
+ *                  is filled with NaN, so that the mistake cannot pass for a
+ *                  result.
+ *   query, key     [num_tokens, num_heads * head_size] and [num_tokens,
+ *                  num_kv_heads * head_size], row strides in elements (column
+ *                  slices of a fused qkv row), any alignment; they must not
+ *                  share an element
+ *   cos_sin_cache  [max_position, rot_dim] = cos(rot_dim/2) | sin(rot_dim/2) per
+ *                  row, of table_dtype: PA_DTYPE_F32, or dtype.  Stretched
+ *                  positions and amplitudes for long contexts are a matter of
+ *                  the table.
+ *   interleaved    0: pair i of a head is (i, i + rot_dim/2); else (2i, 2i + 1)
+ *
+ * The first rot_dim elements of each head are rotated (even, <= head_size), in
+ * fp32 and rounded once; pa_rotary_embedding_neox rounds after every operation,
+ * as the reference does, so the two differ in the last bit of 16-bit types.
+ */
+int pa_rotary_embedding(
+    const int64_t* positions, void* query, void* key, const void* cos_sin_cache,
+    int num_tokens, int num_heads, int num_kv_heads, int head_size, int rot_dim,
+    int64_t max_position, int64_t query_stride, int64_t key_stride,
+    int interleaved, int dtype, int table_dtype, void* stream);
+
+/*
+ * An RMS norm of every query and key head, x * rsqrt(mean(x^2) + epsilon) *
+ * weight over its head_size elements, then pa_rotary_embedding: one pass, in
+ * place, fp32 from the load to the one rounding.  query_weight, key_weight:
+ * [head_size] of dtype.  The elements behind rot_dim are normed and not rotated.
+ */
+int pa_qk_norm_rotary_embedding(
+    const int64_t* positions, void* query, void* key, const void* query_weight,
+    const void* key_weight, float epsilon, const void* cos_sin_cache,
+    int num_tokens, int num_heads, int num_kv_heads, int head_size, int rot_dim,
+    int64_t max_position, int64_t query_stride, int64_t key_stride,
+    int interleaved, int dtype, int table_dtype, void* stream);
+
+/*
  * pa_rotary_embedding_neox followed by pa_reshape_and_cache, in one pass where the
  * shapes allow.  Replaces the pair of calls a rotary attention layer makes for the
  * tokens it caches (vllm/model_executor/layers/attention.py:200-206 rotary_embedding_neox,

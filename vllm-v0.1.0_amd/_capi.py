@@ -40,6 +40,8 @@ EXPORTS = (
     "pa_copy_blocks",
     "pa_swap_blocks",
     "pa_rotary_embedding_neox",
+    "pa_rotary_embedding",
+    "pa_qk_norm_rotary_embedding",
     "pa_rms_norm",
     "pa_silu_and_mul",
     "pa_comm_create",
@@ -103,6 +105,12 @@ def _load() -> ctypes.CDLL:
     lib.pa_swap_blocks.restype = i32
     lib.pa_rotary_embedding_neox.argtypes = [vp, vp, vp, vp, i32, i32, i32, i32, i64, i64, i32, vp]
     lib.pa_rotary_embedding_neox.restype = i32
+    lib.pa_rotary_embedding.argtypes = [
+        vp, vp, vp, vp, i32, i32, i32, i32, i32, i64, i64, i64, i32, i32, i32, vp]
+    lib.pa_rotary_embedding.restype = i32
+    lib.pa_qk_norm_rotary_embedding.argtypes = [
+        vp, vp, vp, vp, vp, f32, vp, i32, i32, i32, i32, i32, i64, i64, i64, i32, i32, i32, vp]
+    lib.pa_qk_norm_rotary_embedding.restype = i32
     lib.pa_rms_norm.argtypes = [vp, vp, vp, f32, i32, i32, i32, vp]
     lib.pa_rms_norm.restype = i32
     lib.pa_silu_and_mul.argtypes = [vp, vp, i32, i32, i32, vp]

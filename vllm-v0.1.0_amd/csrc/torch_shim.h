@@ -26,6 +26,13 @@ inline void* current_stream(const torch::Tensor& t) {
 // have no such guard and misbehave when a tensor lives on a GPU that is not current.
 #define PA_DEVICE_GUARD(tensor) const c10::DeviceGuard pa_device_guard_((tensor).device())
 
+// The launch goes by `first`'s device: a tensor of another one would be read through a foreign pointer.
+inline void check_one_device(const char* what, const torch::Tensor& first,
+                             std::initializer_list<const torch::Tensor*> others) {
+  for (const torch::Tensor* t : others)
+    TORCH_CHECK(t->device() == first.device(), what, ": all tensors must be on one device");
+}
+
 inline int dtype_code(const torch::Tensor& t, const char* what) {
   switch (t.scalar_type()) {
     case at::ScalarType::Float: return PA_DTYPE_F32;
