@@ -235,6 +235,84 @@ int pa_append_single_query_cached_kv_attention(
     int plan_ready, int64_t total_context_len, void* stream);
 
 /*
+ * Attention of several new tokens per sequence over the paged cache: a tree of
+ * drafted tokens, a chain (the next tokens of a prompt, or a draft without
+ * branches), or one token.  No counterpart in the reference.
+ *
+ *   out           [num_tokens, num_heads, head_size], dense
+ *   query         the same, row stride q_stride elements, any alignment
+ *   key_cache, value_cache
+ *                 [num_blocks, num_kv_heads, ...] as above; num_heads is a
+ *                 multiple of num_kv_heads, and query heads h * (num_heads /
+ *                 num_kv_heads) ... share kv head h.  The new tokens' keys and
+ *                 values are already in the cache, at the last positions of
+ *                 their sequence's context in the order of their rows
+ *                 (pa_reshape_and_cache puts them there).
+ *   query_starts  [num_seqs + 1] int32, device: sequence s owns the token rows
+ *                 query_starts[s] .. query_starts[s + 1] - 1, T of them (0 too).
+ *                 Rows behind the last sequence are neither read nor written.
+ *   context_lens  [num_seqs] int32, device: positions in the cache, the T new
+ *                 ones included
+ *   tree_mask     [num_tokens, >= max_query_len] bytes, rows mask_stride apart:
+ *                 token row t sees new position i of its sequence where byte
+ *                 (t, i) is not 0.  NULL: i <= t, a chain.  All T see the
+ *                 ctx - T positions before.  A row that sees nothing is zeros.
+ *
+ * out = softmax(scale q . k) . v over what a row sees (no 1e-6 in the
+ * denominator).  Head sizes 64, 80, 96, 128, block sizes 8, 16, 32, all pa_dtype
+ * values; fp32 accumulation and statistics, the weights rounded to the type.
+ * Keys and values in places that a row does not see, and behind the context,
+ * may be anything (infinities, NaN).
+ *
+ * max_context_len and max_query_len bound the sequences' own and size the launch.  A
+ * sequence that exceeds one, has more new tokens than context or more context
+ * than its table, or whose table names a block >= num_blocks, gets NaN in its
+ * rows; nothing outside the given arrays is read or written for it.
+ *
+ * workspace: pa_tree_workspace_bytes(...) bytes of device memory (0: none),
+ * 16-byte aligned, contents irrelevant; two calls that may overlap in time need
+ * one each.
+ */
+size_t pa_tree_workspace_bytes(int num_seqs, int num_heads, int num_kv_heads,
+                               int head_size, int max_context_len,
+                               int max_query_len, int accumulate);
+
+int pa_tree_cached_kv_attention(
+    void* out, const void* query, const void* key_cache, const void* value_cache,
+    float scale, const int32_t* block_tables, const int32_t* context_lens,
+    const int32_t* query_starts, const uint8_t* tree_mask, int64_t mask_stride,
+    int num_seqs, int num_tokens, int num_heads, int num_kv_heads, int head_size,
+    int block_size, int num_blocks, int max_num_blocks_per_seq,
+    int max_context_len, int max_query_len, int64_t q_stride, int dtype,
+    void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * pa_tree_cached_kv_attention of chains that also keeps every position's
+ * attention weight, for pa_evict_cached_kv:
+ *
+ *   weight_cache  [num_blocks, num_kv_heads, block_size] float, 16-byte aligned.
+ *                 weight(pos) += the sum of the softmax weights that the new
+ *                 tokens' rows give pos, over the query heads that share the kv
+ *                 head; the new positions' entries start from 0 (what a block
+ *                 held before it was handed out does not matter).
+ *
+ * A sequence generating one token a step passes T = 1; after a prompt, a call
+ * with its last T tokens as queries gives the earlier positions their first
+ * weights (the caller zeroes those).  Blocks must not be shared by two sequences
+ * of the call, as their sums would race.  The logits take num_seqs * num_heads *
+ * max_query_len * max_context_len * 4 bytes of the workspace.  The sums are made
+ * in one order, whatever the timing.
+ */
+int pa_cached_kv_attention_accumulate(
+    void* out, const void* query, const void* key_cache, const void* value_cache,
+    float* weight_cache, float scale, const int32_t* block_tables,
+    const int32_t* context_lens, const int32_t* query_starts, int num_seqs,
+    int num_tokens, int num_heads, int num_kv_heads, int head_size,
+    int block_size, int num_blocks, int max_num_blocks_per_seq,
+    int max_context_len, int max_query_len, int64_t q_stride, int dtype,
+    void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * Scatter new key/value vectors into the paged caches.
  * Replaces reshape_and_cache (csrc/cache_kernels.cu:186-224; kernel :143-182).
  *

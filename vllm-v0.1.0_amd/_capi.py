@@ -34,6 +34,9 @@ EXPORTS = (
     "pa_append_single_query_cached_kv_attention",
     "pa_decode_workspace_bytes",
     "pa_multi_query_kv_attention",
+    "pa_tree_workspace_bytes",
+    "pa_tree_cached_kv_attention",
+    "pa_cached_kv_attention_accumulate",
     "pa_reshape_and_cache",
     "pa_rotary_embedding_neox_reshape_and_cache",
     "pa_gather_cached_kv",
@@ -93,6 +96,16 @@ def _load() -> ctypes.CDLL:
     lib.pa_decode_workspace_bytes.restype = ctypes.c_size_t
     lib.pa_multi_query_kv_attention.argtypes = [vp, vp, vp, vp, vp, i32, i32, i32, f32, i64, i64, i64, i32, vp]
     lib.pa_multi_query_kv_attention.restype = i32
+    lib.pa_tree_workspace_bytes.argtypes = [i32] * 7
+    lib.pa_tree_workspace_bytes.restype = ctypes.c_size_t
+    lib.pa_tree_cached_kv_attention.argtypes = [
+        vp, vp, vp, vp, f32, vp, vp, vp, vp, i64, i32, i32, i32, i32, i32, i32, i32, i32, i32, i32, i64, i32, vp,
+        ctypes.c_size_t, vp]
+    lib.pa_tree_cached_kv_attention.restype = i32
+    lib.pa_cached_kv_attention_accumulate.argtypes = [
+        vp, vp, vp, vp, vp, f32, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, i32, i32, i32, i64, i32, vp,
+        ctypes.c_size_t, vp]
+    lib.pa_cached_kv_attention_accumulate.restype = i32
     for fn in (lib.pa_reshape_and_cache, lib.pa_gather_cached_kv):
         fn.argtypes = [vp, vp, vp, vp, vp, i32, i32, i32, i32, i64, i64, i32, vp]
         fn.restype = i32

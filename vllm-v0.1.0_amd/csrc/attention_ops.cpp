@@ -174,6 +174,139 @@ void multi_query_kv_attention(
                what);
 }
 
+// Not part of the reference's module: several new tokens per sequence over the paged cache, whose keys
+// and values reshape_and_cache has put at the end of their contexts.  num_kv_heads is the caches'.
+struct TreeShape {
+  int num_seqs, num_tokens, num_heads, num_kv_heads, head_size, num_blocks, dtype;
+};
+
+TreeShape check_tree_args(const char* what, const torch::Tensor& out, const torch::Tensor& query,
+                          const torch::Tensor& key_cache, const torch::Tensor& value_cache,
+                          const torch::Tensor& block_tables, const torch::Tensor& context_lens,
+                          const torch::Tensor& query_starts, int64_t block_size, int64_t max_context_len,
+                          int64_t max_query_len) {
+  using namespace pa_shim;
+  TORCH_CHECK(query.is_cuda() && out.is_cuda() && key_cache.is_cuda() && value_cache.is_cuda() && block_tables.is_cuda() &&
+                  context_lens.is_cuda() && query_starts.is_cuda(),
+              what, ": all tensors must be on the GPU");
+  check_one_device(what, query, {&out, &key_cache, &value_cache, &block_tables, &context_lens, &query_starts});
+  TreeShape sh;
+  sh.dtype = dtype_code(query, what);
+  TORCH_CHECK(out.scalar_type() == query.scalar_type() && key_cache.scalar_type() == query.scalar_type() &&
+                  value_cache.scalar_type() == query.scalar_type(),
+              what, ": out, query, key_cache and value_cache must share one data type");
+  check_token_rows(query, "query");
+  TORCH_CHECK(out.dim() == 3 && out.is_contiguous() && out.sizes() == query.sizes(), what,
+              ": out must be contiguous and shaped like query");
+  TORCH_CHECK(key_cache.dim() == 5 && value_cache.dim() == 4 && key_cache.is_contiguous() && value_cache.is_contiguous(),
+              what, ": key_cache must be a contiguous 5-d tensor and value_cache a contiguous 4-d tensor");
+  TORCH_CHECK(block_tables.scalar_type() == at::ScalarType::Int && context_lens.scalar_type() == at::ScalarType::Int &&
+                  query_starts.scalar_type() == at::ScalarType::Int,
+              what, ": block_tables, context_lens and query_starts must be int32");
+  TORCH_CHECK(block_tables.dim() == 2 && block_tables.is_contiguous() && context_lens.is_contiguous() &&
+                  query_starts.is_contiguous(),
+              what, ": block_tables must be a contiguous 2-d tensor, context_lens and query_starts contiguous");
+  TORCH_CHECK(context_lens.numel() == block_tables.size(0) && query_starts.numel() == block_tables.size(0) + 1, what,
+              ": block_tables, context_lens and query_starts do not match in the number of sequences");
+  const int64_t x = 16 / query.element_size(), dim = query.size(2), kv = value_cache.size(1);
+  TORCH_CHECK(value_cache.size(2) == dim && value_cache.size(3) == block_size, what,
+              ": value_cache shape does not match [num_blocks, num_kv_heads, ", dim, ", ", block_size, "]");
+  TORCH_CHECK(key_cache.size(0) == value_cache.size(0) && key_cache.size(1) == kv && key_cache.size(2) * x == dim &&
+                  key_cache.size(3) == block_size && key_cache.size(4) == x,
+              what, ": key_cache shape does not match value_cache");
+  TORCH_CHECK(max_context_len >= 0 && max_context_len <= INT32_MAX && max_query_len >= 0 && max_query_len <= INT32_MAX, what,
+              ": max_context_len or max_query_len out of range");
+  TORCH_CHECK(query.size(0) <= INT32_MAX && value_cache.size(0) <= INT32_MAX && block_tables.size(1) <= INT32_MAX &&
+                  block_tables.size(0) <= INT32_MAX,
+              what, ": too many tokens or blocks");
+  sh.num_seqs = block_tables.size(0);
+  sh.num_tokens = query.size(0);
+  sh.num_heads = query.size(1);
+  sh.num_kv_heads = kv;
+  sh.head_size = dim;
+  sh.num_blocks = value_cache.size(0);
+  return sh;
+}
+
+// The scratch comes from torch's caching allocator on the current stream and goes back as soon as the
+// launches are queued (as in single_query_cached_kv_attention).
+torch::Tensor tree_workspace(const torch::Tensor& query, const TreeShape& sh, int max_context_len, int max_query_len,
+                             bool accumulate, size_t* bytes) {
+  *bytes = pa_tree_workspace_bytes(sh.num_seqs, sh.num_heads, sh.num_kv_heads, sh.head_size, max_context_len, max_query_len,
+                                   accumulate);
+  return *bytes ? torch::empty({static_cast<int64_t>(*bytes)}, query.options().dtype(torch::kUInt8)) : torch::Tensor();
+}
+
+void tree_cached_kv_attention(
+    const torch::Tensor& out,           // [num_tokens, num_heads, head_size]
+    const torch::Tensor& query,         // [num_tokens, num_heads, head_size]
+    const torch::Tensor& key_cache,     // [num_blocks, num_kv_heads, head_size/x, block_size, x]
+    const torch::Tensor& value_cache,   // [num_blocks, num_kv_heads, head_size, block_size]
+    double scale,
+    const torch::Tensor& block_tables,  // [num_seqs, max_num_blocks_per_seq]
+    const torch::Tensor& context_lens,  // [num_seqs], the new tokens included
+    const torch::Tensor& query_starts,  // [num_seqs + 1]
+    const std::optional<torch::Tensor>& tree_mask,  // [num_tokens, >= max_query_len] bool or uint8; None: chains
+    int64_t block_size, int64_t max_context_len, int64_t max_query_len) {
+  using namespace pa_shim;
+  const char* what = "tree_cached_kv_attention";
+  const TreeShape sh = check_tree_args(what, out, query, key_cache, value_cache, block_tables, context_lens, query_starts,
+                                       block_size, max_context_len, max_query_len);
+  const uint8_t* mask = nullptr;
+  int64_t mask_stride = 0;
+  if (tree_mask.has_value()) {
+    const torch::Tensor& t = *tree_mask;
+    TORCH_CHECK(t.device() == query.device(), what, ": all tensors must be on one device");
+    TORCH_CHECK(t.scalar_type() == at::ScalarType::Bool || t.scalar_type() == at::ScalarType::Byte, what,
+                ": tree_mask must be bool or uint8");
+    TORCH_CHECK(t.dim() == 2 && t.size(0) >= query.size(0) && t.size(1) >= max_query_len, what,
+                ": tree_mask must be [num_tokens, at least max_query_len]");
+    TORCH_CHECK(t.numel() == 0 || ((t.size(1) == 1 || t.stride(1) == 1) && t.stride(0) >= 0), what,
+                ": tree_mask must be dense in its last dimension");
+    mask = static_cast<const uint8_t*>(t.data_ptr());
+    mask_stride = t.stride(0);
+  }
+  PA_DEVICE_GUARD(query);
+  size_t bytes;
+  const torch::Tensor ws = tree_workspace(query, sh, max_context_len, max_query_len, false, &bytes);
+  check_status(pa_tree_cached_kv_attention(
+                   out.data_ptr(), query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), static_cast<float>(scale),
+                   block_tables.data_ptr<int>(), context_lens.data_ptr<int>(), query_starts.data_ptr<int>(), mask, mask_stride,
+                   sh.num_seqs, sh.num_tokens, sh.num_heads, sh.num_kv_heads, sh.head_size, static_cast<int>(block_size),
+                   sh.num_blocks, static_cast<int>(block_tables.size(1)), static_cast<int>(max_context_len),
+                   static_cast<int>(max_query_len), query.stride(0), sh.dtype, bytes ? ws.data_ptr() : nullptr, bytes,
+                   current_stream(query)),
+               what);
+}
+
+void cached_kv_attention_accumulate(
+    const torch::Tensor& out, const torch::Tensor& query, const torch::Tensor& key_cache, const torch::Tensor& value_cache,
+    const torch::Tensor& weight_cache,  // [num_blocks, num_kv_heads, block_size] float32
+    double scale, const torch::Tensor& block_tables, const torch::Tensor& context_lens, const torch::Tensor& query_starts,
+    int64_t block_size, int64_t max_context_len, int64_t max_query_len) {
+  using namespace pa_shim;
+  const char* what = "cached_kv_attention_accumulate";
+  const TreeShape sh = check_tree_args(what, out, query, key_cache, value_cache, block_tables, context_lens, query_starts,
+                                       block_size, max_context_len, max_query_len);
+  TORCH_CHECK(weight_cache.device() == query.device(), what, ": all tensors must be on one device");
+  TORCH_CHECK(weight_cache.scalar_type() == at::ScalarType::Float && weight_cache.is_contiguous() && weight_cache.dim() == 3 &&
+                  weight_cache.size(0) == sh.num_blocks && weight_cache.size(1) == sh.num_kv_heads &&
+                  weight_cache.size(2) == block_size,
+              what, ": weight_cache must be a contiguous float32 [num_blocks, num_kv_heads, block_size] tensor");
+  PA_DEVICE_GUARD(query);
+  size_t bytes;
+  const torch::Tensor ws = tree_workspace(query, sh, max_context_len, max_query_len, true, &bytes);
+  check_status(pa_cached_kv_attention_accumulate(
+                   out.data_ptr(), query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(),
+                   weight_cache.data_ptr<float>(), static_cast<float>(scale), block_tables.data_ptr<int>(),
+                   context_lens.data_ptr<int>(), query_starts.data_ptr<int>(), sh.num_seqs, sh.num_tokens, sh.num_heads,
+                   sh.num_kv_heads, sh.head_size, static_cast<int>(block_size), sh.num_blocks,
+                   static_cast<int>(block_tables.size(1)), static_cast<int>(max_context_len),
+                   static_cast<int>(max_query_len), query.stride(0), sh.dtype, bytes ? ws.data_ptr() : nullptr, bytes,
+                   current_stream(query)),
+               what);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -188,4 +321,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "that ends with it, in one launch");
   m.def("multi_query_kv_attention", &multi_query_kv_attention,
         "Causal self-attention inside each prompt of a flat token batch (MI355X matrix-core kernel)");
+  m.def("tree_cached_kv_attention", &tree_cached_kv_attention,
+        "Attention of several new tokens per sequence (a tree by its mask, or a chain) over the paged cache");
+  m.def("cached_kv_attention_accumulate", &cached_kv_attention_accumulate,
+        "Attention of new tokens over the paged cache that adds every position's weight to weight_cache");
 }

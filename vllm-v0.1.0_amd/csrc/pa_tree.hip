@@ -1,0 +1,285 @@
+// Cached attention of several queries per sequence: the entry points, the launch
+// plan, the kernel that joins context partitions and adds up the weight cache.
+// The attention kernel itself is in pa_tree_kernel.h.
+#include <math.h>
+
+#include <algorithm>
+
+#include "pa_tree.h"
+
+namespace pa {
+namespace {
+
+// ---- joining partitions, and the weight cache -----------------------------------------------
+//
+// Workgroups below join_groups: a wave to a row, out = sum_p 2^(m_p - m) acc_p / sum_p 2^(m_p - m) l_p.
+// The others: 1024 positions of a (sequence, kv head) each, 4 to a lane, w(pos) += sum over rows
+// 2^(logit - m) / l with l from before the weights' rounding; positions of the new tokens start from 0.
+// Neither waits for the other: each makes the row statistics it needs from the partitions' own.
+// Bound by the logits' read for long contexts (4 bytes a position and row next to the head's
+// 512 of keys and values), by the launch for short ones.
+constexpr int kChunk = 1024;
+constexpr int kStatRows = 256;
+
+template <typename T>
+__device__ __forceinline__ void join_row(const TreeArgs& a, int D, int64_t row_id, int lane) {
+  const int64_t per_seq = (int64_t)a.max_query * a.num_heads;
+  const int seq = (int)(row_id / per_seq);
+  const int rest = (int)(row_id - seq * per_seq);
+  const int query = rest / a.num_heads, h = rest - query * a.num_heads;
+  const TreeSeq sq = tree_seq(a, seq);
+  if (sq.bad || query >= sq.queries) return;
+  const int head = h / a.group, row = query * a.group + (h - head * a.group);
+  float m = -INFINITY, l = 0.f;
+  if (lane < sq.parts) {
+    const f32x4 st = *reinterpret_cast<const f32x4*>(a.ml + tree_row(a, seq, head, lane, row) * 4);
+    m = st[0];
+    l = st[1];
+  }
+  float high = m;
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) high = fmaxf(high, __shfl_xor(high, off));
+  const float f = lane < sq.parts ? __builtin_amdgcn_exp2f(m - high) : 0.f;
+  float sum = l * f;
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) sum += __shfl_xor(sum, off);
+  const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+  const float* acc = a.acc + tree_row(a, seq, head, 0, row) * D;
+  const int64_t next = (int64_t)a.max_rows * D;
+  T* op = static_cast<T*>(a.out) + ((int64_t)(sq.first + query) * a.num_heads + h) * D;
+  // every lane takes part (the factors come from other lanes), those past the head size on its first elements;
+  // four partitions' sums are in flight at once, those past the last are the last again with a factor of 0
+  const int d = 2 * lane, at = d < D ? d : 0;
+  float x = 0.f, y = 0.f;
+  for (int p = 0; p < sq.parts; p += 4) {
+    float2 v[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) v[i] = *reinterpret_cast<const float2*>(acc + (p + i < sq.parts ? p + i : sq.parts - 1) * next + at);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const float fp = __shfl(f, p + i < sq.parts ? p + i : sq.parts - 1);
+      x = __builtin_fmaf(v[i].x, p + i < sq.parts ? fp : 0.f, x);
+      y = __builtin_fmaf(v[i].y, p + i < sq.parts ? fp : 0.f, y);
+    }
+  }
+  if (d < D) {
+    op[d] = (T)(x * inv);
+    op[d + 1] = (T)(y * inv);
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) pa_tree_join_kernel(const TreeArgs a, const int D, const unsigned join_groups,
+                                                           const int chunks) {
+  if (blockIdx.x < join_groups) {
+    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row < (int64_t)a.num_seqs * a.max_query * a.num_heads) join_row<T>(a, D, row, threadIdx.x & 63);
+    return;
+  }
+  const unsigned id = blockIdx.x - join_groups;
+  const int chunk = (int)(id % (unsigned)chunks);
+  const int head = (int)(id / (unsigned)chunks % (unsigned)a.num_kv_heads);
+  const int seq = (int)(id / (unsigned)chunks / (unsigned)a.num_kv_heads);
+  const TreeSeq sq = tree_seq(a, seq);
+  if (sq.bad || sq.rows == 0 || chunk * kChunk >= sq.ctx) return;
+  __shared__ float sm_m[kStatRows], sm_inv[kStatRows];
+  const int pos = chunk * kChunk + (int)threadIdx.x * 4;
+  f32x4 w = {0, 0, 0, 0};
+  const float* lg = a.logits + ((int64_t)seq * a.num_kv_heads + head) * a.max_rows * a.logit_stride + pos;
+  for (int r0 = 0; r0 < sq.rows; r0 += kStatRows) {
+    const int n = sq.rows - r0 < kStatRows ? sq.rows - r0 : kStatRows;
+    __syncthreads();
+    if ((int)threadIdx.x < n) {
+      float high = -INFINITY, sum = 0.f;
+      for (int p = 0; p < sq.parts; p++) high = fmaxf(high, a.ml[tree_row(a, seq, head, p, r0 + threadIdx.x) * 4]);
+      for (int p = 0; p < sq.parts; p++) {
+        const float* st = a.ml + tree_row(a, seq, head, p, r0 + threadIdx.x) * 4;
+        sum = __builtin_fmaf(st[2], __builtin_amdgcn_exp2f(st[0] - high), sum);
+      }
+      sm_m[threadIdx.x] = high;
+      sm_inv[threadIdx.x] = sum == 0.f ? 0.f : 1.0f / sum;
+    }
+    __syncthreads();
+    if (pos < sq.ctx) {
+#pragma unroll 4
+      for (int r = 0; r < n; r++) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(lg + (int64_t)(r0 + r) * a.logit_stride);
+#pragma unroll
+        for (int i = 0; i < 4; i++) w[i] = __builtin_fmaf(__builtin_amdgcn_exp2f(x[i] - sm_m[r]), sm_inv[r], w[i]);
+      }
+    }
+  }
+  if (pos >= sq.ctx) return;
+  const int block = a.tables[(int64_t)seq * a.table_width + (pos >> a.block_bits)];
+  if ((unsigned)block >= (unsigned)a.num_blocks) return;
+  // four positions of one block: block sizes are multiples of 8
+  float* wp = a.weights + (((int64_t)block * a.num_kv_heads + head) << a.block_bits) + (pos & ((1 << a.block_bits) - 1));
+  const f32x4 old = *reinterpret_cast<const f32x4*>(wp);
+  const int fresh = sq.ctx - sq.queries;
+#pragma unroll
+  for (int i = 0; i < 4; i++) w[i] = pos + i >= sq.ctx ? old[i] : (pos + i >= fresh ? w[i] : old[i] + w[i]);
+  *reinterpret_cast<f32x4*>(wp) = w;
+}
+
+// ---- launch plan ---------------------------------------------------------------------------------
+
+struct TreePlan {
+  int parts, part_len, row_tiles;
+  int64_t max_rows, logit_stride;
+  size_t ml_bytes, acc_bytes, logit_bytes;
+  size_t bytes() const { return ml_bytes + acc_bytes + logit_bytes; }
+};
+
+constexpr int kChipCUs = 256;
+constexpr int kPartTokens = 128;   // a partition is a multiple of this
+constexpr int kMaxParts = 64;      // the join gives each a lane
+
+TreePlan tree_plan(int num_seqs, int num_heads, int num_kv_heads, int head_size, int max_ctx, int max_query, bool accumulate) {
+  TreePlan p;
+  p.max_rows = (int64_t)max_query * (num_heads / num_kv_heads);
+  const int rows = tree_form(p.max_rows).rows();
+  p.row_tiles = (int)std::max<int64_t>(1, (p.max_rows + rows - 1) / rows);
+  const int64_t groups = std::max<int64_t>(1, (int64_t)num_seqs * num_kv_heads * p.row_tiles);
+  // Partitions until there are three workgroups to a CU, none shorter than two steps of every wave.
+  const int64_t want = (3 * kChipCUs + groups - 1) / groups;
+  const int64_t most = std::max<int64_t>(1, (max_ctx + 255) / 256);
+  const int64_t parts = std::max<int64_t>(1, std::min<int64_t>({want, most, (int64_t)kMaxParts}));
+  const int64_t len = (max_ctx + parts - 1) / parts;
+  p.part_len = (int)std::max<int64_t>(kPartTokens, (len + kPartTokens - 1) / kPartTokens * kPartTokens);
+  p.parts = (int)std::max<int64_t>(1, ((int64_t)max_ctx + p.part_len - 1) / p.part_len);
+  const size_t cells = (size_t)num_seqs * num_kv_heads * p.parts * p.max_rows;
+  p.ml_bytes = p.parts > 1 || accumulate ? cells * 16 : 0;
+  p.acc_bytes = p.parts > 1 ? cells * head_size * 4 : 0;
+  p.logit_stride = ((int64_t)max_ctx + 31) / 32 * 32;
+  p.logit_bytes = accumulate ? (size_t)num_seqs * num_kv_heads * p.max_rows * p.logit_stride * 4 : 0;
+  return p;
+}
+
+int tree_entry(const char* what, void* out, const void* query, const void* key_cache, const void* value_cache,
+               float* weight_cache, bool accumulate, float scale, const int32_t* block_tables, const int32_t* context_lens,
+               const int32_t* query_starts, const uint8_t* tree_mask, int64_t mask_stride, int num_seqs, int num_tokens,
+               int num_heads, int num_kv_heads, int head_size, int block_size, int num_blocks, int max_num_blocks_per_seq,
+               int max_context_len, int max_query_len, int64_t q_stride, int dtype, void* workspace,
+               size_t workspace_bytes, void* stream) {
+  clear_error();
+  if (dtype != PA_DTYPE_F32 && dtype != PA_DTYPE_F16 && dtype != PA_DTYPE_BF16)
+    return fail(PA_ERR_UNSUPPORTED, "%s: unsupported data type code: %d", what, dtype);
+  if (head_size != 64 && head_size != 80 && head_size != 96 && head_size != 128)
+    return fail(PA_ERR_UNSUPPORTED, "%s: unsupported head size: %d", what, head_size);
+  if (block_size != 8 && block_size != 16 && block_size != 32)
+    return fail(PA_ERR_UNSUPPORTED, "%s: unsupported block size: %d", what, block_size);
+  PA_REQUIRE(num_seqs >= 0 && num_tokens >= 0 && num_heads >= 0 && num_kv_heads >= 0 && num_blocks >= 0 &&
+                 max_num_blocks_per_seq >= 0 && max_context_len >= 0 && max_query_len >= 0,
+             "%s: negative size", what);
+  if (num_seqs == 0 || num_tokens == 0 || num_heads == 0 || max_query_len == 0) return PA_OK;
+  PA_REQUIRE(num_kv_heads > 0 && num_heads % num_kv_heads == 0, "%s: num_heads %d is no multiple of num_kv_heads %d", what,
+             num_heads, num_kv_heads);
+  PA_REQUIRE(out && query && key_cache && value_cache && block_tables && context_lens && query_starts &&
+                 (weight_cache || !accumulate),
+             "%s: null pointer argument", what);
+  PA_REQUIRE(aligned16(out) && aligned16(key_cache) && aligned16(value_cache) && aligned16(weight_cache),
+             "%s: out and the caches must be 16-byte aligned", what);
+  PA_REQUIRE(isfinite(scale), "%s: scale must be finite", what);
+  PA_REQUIRE(num_tokens == 1 || q_stride >= (int64_t)num_heads * head_size, "%s: query row stride is shorter than a token row", what);
+  PA_REQUIRE((int64_t)max_num_blocks_per_seq * block_size >= max_context_len,
+             "%s: block tables of %d blocks cannot hold max_context_len %d", what, max_num_blocks_per_seq, max_context_len);
+  PA_REQUIRE(max_query_len <= max_context_len, "%s: max_query_len %d exceeds max_context_len %d (which counts the new tokens)",
+             what, max_query_len, max_context_len);
+  PA_REQUIRE(max_context_len <= (1 << 30), "%s: max_context_len %d is too large", what, max_context_len);
+  PA_REQUIRE(tree_mask == nullptr || mask_stride >= 0, "%s: negative mask stride", what);
+  PA_REQUIRE(num_blocks > 0, "%s: the caches have no blocks", what);
+  const TreePlan p = tree_plan(num_seqs, num_heads, num_kv_heads, head_size, max_context_len, max_query_len, accumulate);
+  const int64_t items = (int64_t)num_seqs * num_kv_heads * p.parts;
+  const int64_t grid = (items + 7) / 8 * 8 * p.row_tiles;
+  const int64_t join_groups = p.parts > 1 ? ((int64_t)num_seqs * max_query_len * num_heads + 3) / 4 : 0;
+  const int chunks = (max_context_len + kChunk - 1) / kChunk;
+  const int64_t join_grid = join_groups + (accumulate ? (int64_t)num_seqs * num_kv_heads * chunks : 0);
+  PA_REQUIRE(grid <= 0x7fffffff && join_grid <= 0x7fffffff && p.max_rows <= 0x7fffffff, "%s: too many rows for one launch", what);
+  PA_REQUIRE(p.bytes() == 0 || (workspace && aligned16(workspace) && workspace_bytes >= p.bytes()),
+             "%s: workspace of %zu bytes, 16-byte aligned, needed", what, p.bytes());
+
+  TreeArgs a = {};
+  a.out = out;
+  a.q = query;
+  a.kc = static_cast<const char*>(key_cache);
+  a.vc = static_cast<const char*>(value_cache);
+  a.tables = block_tables;
+  a.ctx = context_lens;
+  a.starts = query_starts;
+  a.mask = tree_mask;
+  a.weights = accumulate ? weight_cache : nullptr;
+  char* ws = static_cast<char*>(workspace);
+  a.ml = reinterpret_cast<float*>(ws);
+  a.acc = reinterpret_cast<float*>(ws + p.ml_bytes);
+  a.logits = reinterpret_cast<float*>(ws + p.ml_bytes + p.acc_bytes);
+  a.q_stride = q_stride;
+  a.mask_stride = mask_stride;
+  a.logit_stride = p.logit_stride;
+  a.c = scale == 0.f ? 1.f : fabsf(scale) * 1.44269504088896340736f;
+  a.q_mode = scale == 0.f ? 2 : (scale < 0.f ? 1 : 0);
+  a.num_seqs = num_seqs;
+  a.num_tokens = num_tokens;
+  a.num_heads = num_heads;
+  a.num_kv_heads = num_kv_heads;
+  a.group = num_heads / num_kv_heads;
+  a.num_blocks = num_blocks;
+  a.block_bits = block_size == 8 ? 3 : (block_size == 16 ? 4 : 5);
+  a.table_width = max_num_blocks_per_seq;
+  a.max_ctx = max_context_len;
+  a.max_query = max_query_len;
+  a.max_rows = (int)p.max_rows;
+  a.parts = p.parts;
+  a.part_len = p.part_len;
+  a.row_tiles = p.row_tiles;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  int rc;
+  switch (dtype) {
+    case PA_DTYPE_F32: rc = tree_launch_f32(a, head_size, (unsigned)grid, st); break;
+    case PA_DTYPE_F16: rc = tree_launch_f16(a, head_size, (unsigned)grid, st); break;
+    default: rc = tree_launch_bf16(a, head_size, (unsigned)grid, st); break;
+  }
+  if (rc != PA_OK || join_grid == 0) return rc;
+  const dim3 jg((unsigned)join_grid), jb(256);
+  switch (dtype) {
+    case PA_DTYPE_F32: hipLaunchKernelGGL((pa_tree_join_kernel<float>), jg, jb, 0, st, a, head_size, (unsigned)join_groups, chunks); break;
+    case PA_DTYPE_F16: hipLaunchKernelGGL((pa_tree_join_kernel<_Float16>), jg, jb, 0, st, a, head_size, (unsigned)join_groups, chunks); break;
+    default: hipLaunchKernelGGL((pa_tree_join_kernel<__bf16>), jg, jb, 0, st, a, head_size, (unsigned)join_groups, chunks); break;
+  }
+  PA_CHECK_LAUNCH(what);
+  return PA_OK;
+}
+
+}  // namespace
+}  // namespace pa
+
+extern "C" size_t pa_tree_workspace_bytes(int num_seqs, int num_heads, int num_kv_heads, int head_size, int max_context_len,
+                                          int max_query_len, int accumulate) {
+  if (num_seqs <= 0 || num_heads <= 0 || num_kv_heads <= 0 || head_size <= 0 || max_context_len <= 0 || max_query_len <= 0 ||
+      num_heads % num_kv_heads != 0)
+    return 0;
+  return pa::tree_plan(num_seqs, num_heads, num_kv_heads, head_size, max_context_len, max_query_len, accumulate != 0).bytes();
+}
+
+extern "C" int pa_tree_cached_kv_attention(
+    void* out, const void* query, const void* key_cache, const void* value_cache, float scale, const int32_t* block_tables,
+    const int32_t* context_lens, const int32_t* query_starts, const uint8_t* tree_mask, int64_t mask_stride, int num_seqs,
+    int num_tokens, int num_heads, int num_kv_heads, int head_size, int block_size, int num_blocks,
+    int max_num_blocks_per_seq, int max_context_len, int max_query_len, int64_t q_stride, int dtype, void* workspace,
+    size_t workspace_bytes, void* stream) {
+  return pa::tree_entry("pa_tree_cached_kv_attention", out, query, key_cache, value_cache, nullptr, false, scale, block_tables,
+                        context_lens, query_starts, tree_mask, mask_stride, num_seqs, num_tokens, num_heads, num_kv_heads,
+                        head_size, block_size, num_blocks, max_num_blocks_per_seq, max_context_len, max_query_len, q_stride,
+                        dtype, workspace, workspace_bytes, stream);
+}
+
+extern "C" int pa_cached_kv_attention_accumulate(
+    void* out, const void* query, const void* key_cache, const void* value_cache, float* weight_cache, float scale,
+    const int32_t* block_tables, const int32_t* context_lens, const int32_t* query_starts, int num_seqs, int num_tokens,
+    int num_heads, int num_kv_heads, int head_size, int block_size, int num_blocks, int max_num_blocks_per_seq,
+    int max_context_len, int max_query_len, int64_t q_stride, int dtype, void* workspace, size_t workspace_bytes,
+    void* stream) {
+  return pa::tree_entry("pa_cached_kv_attention_accumulate", out, query, key_cache, value_cache, weight_cache, true, scale,
+                        block_tables, context_lens, query_starts, nullptr, 0, num_seqs, num_tokens, num_heads, num_kv_heads,
+                        head_size, block_size, num_blocks, max_num_blocks_per_seq, max_context_len, max_query_len, q_stride,
+                        dtype, workspace, workspace_bytes, stream);
+}
