@@ -345,6 +345,42 @@ int pa_gather_cached_kv(
     void* stream);
 
 /*
+ * Drops the positions with the least accumulated weight from long sequences, in
+ * place.  No counterpart in the reference.  Of every (sequence, kv head) with
+ * more than `budget` positions there stay the last num_recent and, of those
+ * before, the budget - num_recent of the largest weight_cache entry (equal ones:
+ * the lowest positions; both zeros are equal, NaN is larger than all).  They keep
+ * their order and move to slots 0 .. budget - 1 of the sequence's blocks, in all
+ * three caches; each head chooses for itself.  Slots from budget on stay as they
+ * are: the caller takes min(context_len, budget) as the new context length and
+ * may free the blocks behind it.  Rotated keys keep their rotation; the next
+ * token's position is the sequence's true one, its slot the next free one.
+ *
+ *   weight_cache    [num_blocks, num_kv_heads, block_size] float, as
+ *                   pa_cached_kv_attention_accumulate fills it
+ *   kept_positions  [num_seqs, num_kv_heads, budget] int32, output: the positions
+ *                   that stay, rising, -1 behind the last
+ *
+ * A sequence within the budget is left as it is.  One whose context exceeds
+ * max_context_len or its table, or whose table names a block outside the cache,
+ * is left as it is too, all its kept_positions -1.  Blocks that the call writes
+ * must not be shared: two sequences' moves would race, and a fork would lose its
+ * positions (copy them first, pa_copy_blocks).  head_size: a multiple of x;
+ * block sizes 8, 16, 32; all pa_dtype values.  workspace: pa_evict_workspace_bytes
+ * of device memory, 16-byte aligned, contents irrelevant.
+ */
+size_t pa_evict_workspace_bytes(int num_seqs, int num_kv_heads,
+                                int max_context_len);
+
+int pa_evict_cached_kv(
+    void* key_cache, void* value_cache, float* weight_cache,
+    const int32_t* block_tables, const int32_t* context_lens,
+    int32_t* kept_positions, int num_seqs, int num_kv_heads, int head_size,
+    int block_size, int num_blocks, int max_num_blocks_per_seq,
+    int max_context_len, int budget, int num_recent, int dtype, void* workspace,
+    size_t workspace_bytes, void* stream);
+
+/*
  * For every layer and every (src, dst) pair copy one key block and one value
  * block inside the same cache tensor.  Replaces copy_blocks
  * (csrc/cache_kernels.cu:82-138; kernel :53-78).

@@ -185,6 +185,58 @@ void gather_cached_kv(torch::Tensor& key, torch::Tensor& value, torch::Tensor& k
                what);
 }
 
+// Not part of the reference's module: keeps the heaviest and the latest positions of every (sequence,
+// kv head) over its budget (kept_positions' last size) and moves them to the front, in place.
+void evict_cached_kv(const torch::Tensor& key_cache,      // [num_blocks, num_kv_heads, head_size/x, block_size, x]
+                     const torch::Tensor& value_cache,    // [num_blocks, num_kv_heads, head_size, block_size]
+                     const torch::Tensor& weight_cache,   // [num_blocks, num_kv_heads, block_size] float32
+                     const torch::Tensor& block_tables,   // [num_seqs, max_num_blocks_per_seq]
+                     const torch::Tensor& context_lens,   // [num_seqs]
+                     const torch::Tensor& kept_positions, // [num_seqs, num_kv_heads, budget] int32, written
+                     int64_t num_recent, int64_t max_context_len) {
+  const char* what = "evict_cached_kv";
+  TORCH_CHECK(key_cache.is_cuda() && value_cache.is_cuda() && weight_cache.is_cuda() && block_tables.is_cuda() &&
+                  context_lens.is_cuda() && kept_positions.is_cuda(),
+              what, ": all tensors must be on the GPU");
+  pa_shim::check_one_device(what, key_cache, {&value_cache, &weight_cache, &block_tables, &context_lens, &kept_positions});
+  const int dtype = dtype_code(key_cache, what);
+  TORCH_CHECK(value_cache.scalar_type() == key_cache.scalar_type(), what, ": key_cache and value_cache must share one data type");
+  TORCH_CHECK(key_cache.dim() == 5 && value_cache.dim() == 4 && key_cache.is_contiguous() && value_cache.is_contiguous(),
+              what, ": key_cache must be a contiguous 5-d tensor and value_cache a contiguous 4-d tensor");
+  const int64_t blocks = value_cache.size(0), heads = value_cache.size(1), dim = value_cache.size(2), block = value_cache.size(3);
+  const int64_t x = 16 / key_cache.element_size();
+  TORCH_CHECK(key_cache.size(0) == blocks && key_cache.size(1) == heads && key_cache.size(2) * x == dim &&
+                  key_cache.size(3) == block && key_cache.size(4) == x,
+              what, ": key_cache shape does not match value_cache");
+  TORCH_CHECK(weight_cache.scalar_type() == at::ScalarType::Float && weight_cache.is_contiguous() && weight_cache.dim() == 3 &&
+                  weight_cache.size(0) == blocks && weight_cache.size(1) == heads && weight_cache.size(2) == block,
+              what, ": weight_cache must be a contiguous float32 [num_blocks, num_kv_heads, block_size] tensor");
+  TORCH_CHECK(block_tables.scalar_type() == at::ScalarType::Int && context_lens.scalar_type() == at::ScalarType::Int &&
+                  kept_positions.scalar_type() == at::ScalarType::Int,
+              what, ": block_tables, context_lens and kept_positions must be int32");
+  TORCH_CHECK(block_tables.dim() == 2 && block_tables.is_contiguous() && context_lens.is_contiguous() &&
+                  kept_positions.is_contiguous(),
+              what, ": block_tables must be a contiguous 2-d tensor, context_lens and kept_positions contiguous");
+  const int64_t seqs = block_tables.size(0);
+  TORCH_CHECK(context_lens.numel() == seqs && kept_positions.dim() == 3 && kept_positions.size(0) == seqs &&
+                  kept_positions.size(1) == heads,
+              what, ": block_tables, context_lens and kept_positions [num_seqs, num_kv_heads, budget] do not match");
+  TORCH_CHECK(max_context_len >= 0 && max_context_len <= INT32_MAX && kept_positions.size(2) <= INT32_MAX && blocks <= INT32_MAX &&
+                  seqs <= INT32_MAX && dim <= INT32_MAX && block_tables.size(1) <= INT32_MAX && num_recent >= 0 && num_recent <= INT32_MAX,
+              what, ": size out of range");
+  PA_DEVICE_GUARD(key_cache);
+  const size_t bytes = pa_evict_workspace_bytes(static_cast<int>(seqs), static_cast<int>(heads), static_cast<int>(max_context_len));
+  const torch::Tensor ws = torch::empty({static_cast<int64_t>(bytes)}, key_cache.options().dtype(torch::kUInt8));
+  check_status(pa_evict_cached_kv(key_cache.data_ptr(), value_cache.data_ptr(), weight_cache.data_ptr<float>(),
+                                  block_tables.data_ptr<int>(), context_lens.data_ptr<int>(), kept_positions.data_ptr<int>(),
+                                  static_cast<int>(seqs), static_cast<int>(heads), static_cast<int>(dim), static_cast<int>(block),
+                                  static_cast<int>(blocks), static_cast<int>(block_tables.size(1)),
+                                  static_cast<int>(max_context_len), static_cast<int>(kept_positions.size(2)),
+                                  static_cast<int>(num_recent), dtype, bytes ? ws.data_ptr() : nullptr, bytes,
+                                  current_stream(key_cache)),
+               what);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -192,6 +244,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("copy_blocks", &copy_blocks, "Copy cache blocks src -> dst inside every layer's key and value cache");
   m.def("reshape_and_cache", &reshape_and_cache, "Scatter new key/value vectors into the paged caches");
   m.def("gather_cached_kv", &gather_cached_kv, "Gather key/value vectors from the paged caches into token rows");
+  m.def("evict_cached_kv", &evict_cached_kv,
+        "Keep the heaviest and the latest positions of every kv head and move them to the front of the sequence's blocks");
   m.def("rotary_embedding_neox_reshape_and_cache", &rotary_embedding_neox_reshape_and_cache,
         "rotary_embedding_neox on query and key in place, then reshape_and_cache of key and value: one pass");
 }
