@@ -54,16 +54,14 @@ __device__ __forceinline__ int64_t tree_row(const TreeArgs& a, int s, int head, 
   return (((int64_t)s * a.num_kv_heads + head) * a.parts + part) * a.max_rows + row;
 }
 
-// Rows of one workgroup for a launch of at most `rows` rows a sequence and kv head, and its form.
-struct TreeForm {
-  int row_tiles_per_wave, row_waves;
-  int rows() const { return 16 * row_tiles_per_wave * row_waves; }
-};
+// The kernel for a launch of at most `rows` rows a sequence and kv head, by the rows of a workgroup.
+enum TreeForm { kTreeFew16 = 16, kTreeFew32 = 32, kTreeMany64 = 64, kTreeMany128 = 128, kTreeMany256 = 256 };
 inline TreeForm tree_form(int64_t rows) {
-  if (rows <= 16) return {1, 1};
-  if (rows <= 32) return {2, 1};
-  if (rows <= 64) return {2, 2};
-  return {2, 4};
+  if (rows <= 16) return kTreeFew16;
+  if (rows <= 32) return kTreeFew32;
+  if (rows <= 64) return kTreeMany64;
+  if (rows <= 128) return kTreeMany128;
+  return kTreeMany256;
 }
 
 // pa_tree_f16.hip, pa_tree_bf16.hip, pa_tree_f32.hip

@@ -28,7 +28,7 @@ __device__ __forceinline__ void join_row(const TreeArgs& a, int D, int64_t row_i
   const int rest = (int)(row_id - seq * per_seq);
   const int query = rest / a.num_heads, h = rest - query * a.num_heads;
   const TreeSeq sq = tree_seq(a, seq);
-  if (sq.bad || query >= sq.queries) return;
+  if (sq.bad || query >= sq.queries || sq.parts == 1) return;  // one partition: the result is there
   const int head = h / a.group, row = query * a.group + (h - head * a.group);
   float m = -INFINITY, l = 0.f;
   if (lane < sq.parts) {
@@ -137,7 +137,7 @@ constexpr int kMaxParts = 64;      // the join gives each a lane
 TreePlan tree_plan(int num_seqs, int num_heads, int num_kv_heads, int head_size, int max_ctx, int max_query, bool accumulate) {
   TreePlan p;
   p.max_rows = (int64_t)max_query * (num_heads / num_kv_heads);
-  const int rows = tree_form(p.max_rows).rows();
+  const int rows = tree_form(p.max_rows);
   p.row_tiles = (int)std::max<int64_t>(1, (p.max_rows + rows - 1) / rows);
   const int64_t groups = std::max<int64_t>(1, (int64_t)num_seqs * num_kv_heads * p.row_tiles);
   // Partitions until there are three workgroups to a CU, none shorter than two steps of every wave.
