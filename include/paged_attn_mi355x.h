@@ -275,7 +275,7 @@ int pa_append_single_query_cached_kv_attention(
  */
 size_t pa_tree_workspace_bytes(int num_seqs, int num_heads, int num_kv_heads,
                                int head_size, int max_context_len,
-                               int max_query_len, int accumulate);
+                               int max_query_len, int accumulate, int dtype);
 
 int pa_tree_cached_kv_attention(
     void* out, const void* query, const void* key_cache, const void* value_cache,
@@ -299,8 +299,9 @@ int pa_tree_cached_kv_attention(
  * A sequence generating one token a step passes T = 1; after a prompt, a call
  * with its last T tokens as queries gives the earlier positions their first
  * weights (the caller zeroes those).  Blocks must not be shared by two sequences
- * of the call, as their sums would race.  The logits take num_seqs * num_heads *
- * max_query_len * max_context_len * 4 bytes of the workspace.  The sums are made
+ * of the call, as their sums would race.  Contexts too long to be read by one
+ * workgroup keep their logits in the workspace: num_seqs * num_heads *
+ * max_query_len * max_context_len * 4 bytes.  The sums are made
  * in one order, whatever the timing.
  */
 int pa_cached_kv_attention_accumulate(

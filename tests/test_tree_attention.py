@@ -455,10 +455,10 @@ def test_c_entry_refuses_without_a_gpu(pkg):
         assert call(acc, mq=0) == c.PA_OK
     assert call(True, w=None) == c.PA_ERR_INVALID_ARGUMENT and "null" in c.last_error()
     assert call(mask=p, ms=-1) == c.PA_ERR_INVALID_ARGUMENT and "mask" in c.last_error()
-    assert c.lib.pa_tree_workspace_bytes(0, 4, 2, 64, 64, 1, 0) == 0
-    assert c.lib.pa_tree_workspace_bytes(2, 4, 3, 64, 64, 1, 1) == 0
-    # the logits alone: 2 sequences x 4 heads x 3 tokens x 64 positions
-    assert c.lib.pa_tree_workspace_bytes(2, 4, 2, 64, 64, 3, 1) >= 2 * 4 * 3 * 64 * 4
+    assert c.lib.pa_tree_workspace_bytes(0, 4, 2, 64, 64, 1, 0, c.PA_DTYPE_F16) == 0
+    assert c.lib.pa_tree_workspace_bytes(2, 4, 3, 64, 64, 1, 1, c.PA_DTYPE_F16) == 0
+    # contexts in partitions: the logits alone are 2 sequences x 4 heads x 3 tokens x 8192 positions
+    assert c.lib.pa_tree_workspace_bytes(2, 4, 2, 64, 8192, 3, 1, c.PA_DTYPE_F16) >= 2 * 4 * 3 * 8192 * 4
 
 
 def test_modules_refuse_cpu_tensors(pkg):

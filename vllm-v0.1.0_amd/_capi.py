@@ -98,7 +98,7 @@ def _load() -> ctypes.CDLL:
     lib.pa_decode_workspace_bytes.restype = ctypes.c_size_t
     lib.pa_multi_query_kv_attention.argtypes = [vp, vp, vp, vp, vp, i32, i32, i32, f32, i64, i64, i64, i32, vp]
     lib.pa_multi_query_kv_attention.restype = i32
-    lib.pa_tree_workspace_bytes.argtypes = [i32] * 7
+    lib.pa_tree_workspace_bytes.argtypes = [i32] * 8
     lib.pa_tree_workspace_bytes.restype = ctypes.c_size_t
     lib.pa_tree_cached_kv_attention.argtypes = [
         vp, vp, vp, vp, f32, vp, vp, vp, vp, i64, i32, i32, i32, i32, i32, i32, i32, i32, i32, i32, i64, i32, vp,

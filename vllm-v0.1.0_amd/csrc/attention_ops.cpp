@@ -233,7 +233,7 @@ TreeShape check_tree_args(const char* what, const torch::Tensor& out, const torc
 torch::Tensor tree_workspace(const torch::Tensor& query, const TreeShape& sh, int max_context_len, int max_query_len,
                              bool accumulate, size_t* bytes) {
   *bytes = pa_tree_workspace_bytes(sh.num_seqs, sh.num_heads, sh.num_kv_heads, sh.head_size, max_context_len, max_query_len,
-                                   accumulate);
+                                   accumulate, sh.dtype);
   return *bytes ? torch::empty({static_cast<int64_t>(*bytes)}, query.options().dtype(torch::kUInt8)) : torch::Tensor();
 }
 

@@ -6,6 +6,8 @@
 
 namespace pa {
 
+constexpr int kPartTokens = 128;  // a context partition is a multiple of this: a step for each of 4 waves
+
 struct TreeArgs {
   void* out;                // [num_tokens, num_heads, head_size]
   const void* q;
@@ -25,13 +27,14 @@ struct TreeArgs {
   int num_seqs, num_tokens, num_heads, num_kv_heads, group;
   int num_blocks, block_bits, table_width;
   int max_ctx, max_query, max_rows;
-  int parts, part_len;      // context partitions of part_len positions
+  int parts, part_len;      // at most so many context partitions, of at most part_len positions
   int row_tiles;            // workgroups along a sequence's rows
+  int form;                 // TreeForm
 };
 
 // What a launch does with one sequence, the same for every kernel that asks.
 struct TreeSeq {
-  int first, queries, rows, ctx, parts;
+  int first, queries, rows, ctx, parts, part_len;
   bool bad;  // the arguments contradict each other: its rows are filled with NaN
 };
 
@@ -45,8 +48,11 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeArgs& a, int s) {
   r.bad = lo < 0 || hi > a.num_tokens || hi < lo || r.queries > a.max_query || r.ctx < r.queries || r.ctx > a.max_ctx ||
           r.ctx > ((int64_t)a.table_width << a.block_bits);
   r.rows = r.queries * a.group;
-  const int p = (r.ctx + a.part_len - 1) / a.part_len;
-  r.parts = p < 1 ? 1 : (p < a.parts ? p : a.parts);
+  // as few partitions as part_len allows, of one length: a last one of any length would leave others waiting
+  const int ctx = r.bad || r.ctx < 1 ? 1 : r.ctx;
+  const int p = (ctx + a.part_len - 1) / a.part_len;
+  r.part_len = ((ctx + p - 1) / p + kPartTokens - 1) / kPartTokens * kPartTokens;
+  r.parts = (ctx + r.part_len - 1) / r.part_len;
   return r;
 }
 
@@ -54,14 +60,38 @@ __device__ __forceinline__ int64_t tree_row(const TreeArgs& a, int s, int head, 
   return (((int64_t)s * a.num_kv_heads + head) * a.parts + part) * a.max_rows + row;
 }
 
+// Whether a workgroup of tile_rows rows has a sequence's logits to itself
+__device__ __forceinline__ bool tree_whole(const TreeSeq& sq, int tile_rows) { return sq.parts == 1 && sq.rows <= tile_rows; }
+
+// Four positions' weights into the weight cache: added, but the new tokens' own start from 0
+__device__ __forceinline__ void add_weights(const TreeArgs& a, const TreeSeq& sq, int seq, int head, int pos, f32x4 w) {
+  const int block = a.tables[(int64_t)seq * a.table_width + (pos >> a.block_bits)];
+  if ((unsigned)block >= (unsigned)a.num_blocks) return;
+  // four positions of one block: block sizes are multiples of 8
+  float* to = a.weights + (((int64_t)block * a.num_kv_heads + head) << a.block_bits) + (pos & ((1 << a.block_bits) - 1));
+  const f32x4 old = *reinterpret_cast<const f32x4*>(to);
+  const int fresh = sq.ctx - sq.queries;
+#pragma unroll
+  for (int i = 0; i < 4; i++) w[i] = pos + i >= sq.ctx ? old[i] : (pos + i >= fresh ? w[i] : old[i] + w[i]);
+  *reinterpret_cast<f32x4*>(to) = w;
+}
+
+// LDS of the few-rows kernel where logits are kept: 48 KiB (three workgroups to a CU), or what joining its
+// waves takes
+constexpr int tree_logit_floats(int head_size, int row_tiles) {
+  const int join = 4 * 16 * row_tiles * (head_size + 4);
+  return join > 12288 ? join : 12288;
+}
+
 // The kernel for a launch of at most `rows` rows a sequence and kv head, by the rows of a workgroup.
-enum TreeForm { kTreeFew16 = 16, kTreeFew32 = 32, kTreeMany64 = 64, kTreeMany128 = 128, kTreeMany256 = 256 };
-inline TreeForm tree_form(int64_t rows) {
+enum TreeForm { kTreeFew16 = 16, kTreeFew32 = 32, kTreeMany64 = 64, kTreeMany128 = 128 };
+inline TreeForm tree_form(int64_t rows, bool accumulate, bool fp32) {
+  const int forced = tuning_int("PA_TREE_FORM", 0);
+  if (forced > 0) return static_cast<TreeForm>(forced);
   if (rows <= 16) return kTreeFew16;
-  if (rows <= 32) return kTreeFew32;
-  if (rows <= 64) return kTreeMany64;
-  if (rows <= 128) return kTreeMany128;
-  return kTreeMany256;
+  if (rows <= 32 || accumulate) return kTreeFew32;  // only the few-rows kernel keeps its logits
+  if (rows <= 64 || fp32) return kTreeMany64;  // fp32 queries of two tiles a wave do not fit its registers
+  return kTreeMany128;
 }
 
 // pa_tree_f16.hip, pa_tree_bf16.hip, pa_tree_f32.hip

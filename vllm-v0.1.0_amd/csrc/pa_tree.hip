@@ -12,7 +12,7 @@ namespace {
 
 // ---- joining partitions, and the weight cache -----------------------------------------------
 //
-// Workgroups below join_groups: a wave to a row, out = sum_p 2^(m_p - m) acc_p / sum_p 2^(m_p - m) l_p.
+// Workgroups below join_groups: head_size / 4 lanes to a row, out = sum_p 2^(m_p - m) acc_p / sum_p 2^(m_p - m) l_p.
 // The others: 1024 positions of a (sequence, kv head) each, 4 to a lane, w(pos) += sum over rows
 // 2^(logit - m) / l with l from before the weights' rounding; positions of the new tokens start from 0.
 // Neither waits for the other: each makes the row statistics it needs from the partitions' own.
@@ -21,8 +21,10 @@ namespace {
 constexpr int kChunk = 1024;
 constexpr int kStatRows = 256;
 
+// A row and 4 of its elements.  One pass, all loads of four partitions on their way at once: the running
+// maximum is raised as in the attention itself.
 template <typename T>
-__device__ __forceinline__ void join_row(const TreeArgs& a, int D, int64_t row_id, int lane) {
+__device__ __forceinline__ void join_row(const TreeArgs& a, int D, int64_t row_id, int d) {
   const int64_t per_seq = (int64_t)a.max_query * a.num_heads;
   const int seq = (int)(row_id / per_seq);
   const int rest = (int)(row_id - seq * per_seq);
@@ -30,50 +32,41 @@ __device__ __forceinline__ void join_row(const TreeArgs& a, int D, int64_t row_i
   const TreeSeq sq = tree_seq(a, seq);
   if (sq.bad || query >= sq.queries || sq.parts == 1) return;  // one partition: the result is there
   const int head = h / a.group, row = query * a.group + (h - head * a.group);
-  float m = -INFINITY, l = 0.f;
-  if (lane < sq.parts) {
-    const f32x4 st = *reinterpret_cast<const f32x4*>(a.ml + tree_row(a, seq, head, lane, row) * 4);
-    m = st[0];
-    l = st[1];
-  }
-  float high = m;
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) high = fmaxf(high, __shfl_xor(high, off));
-  const float f = lane < sq.parts ? __builtin_amdgcn_exp2f(m - high) : 0.f;
-  float sum = l * f;
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) sum += __shfl_xor(sum, off);
-  const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-  const float* acc = a.acc + tree_row(a, seq, head, 0, row) * D;
-  const int64_t next = (int64_t)a.max_rows * D;
-  T* op = static_cast<T*>(a.out) + ((int64_t)(sq.first + query) * a.num_heads + h) * D;
-  // every lane takes part (the factors come from other lanes), those past the head size on its first elements;
-  // four partitions' sums are in flight at once, those past the last are the last again with a factor of 0
-  const int d = 2 * lane, at = d < D ? d : 0;
-  float x = 0.f, y = 0.f;
+  const int64_t first = tree_row(a, seq, head, 0, row);
+  float high = -INFINITY, sum = 0.f;
+  f32x4 x = {0, 0, 0, 0};
   for (int p = 0; p < sq.parts; p += 4) {
-    float2 v[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) v[i] = *reinterpret_cast<const float2*>(acc + (p + i < sq.parts ? p + i : sq.parts - 1) * next + at);
+    float2 st[4];
+    f32x4 v[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-      const float fp = __shfl(f, p + i < sq.parts ? p + i : sq.parts - 1);
-      x = __builtin_fmaf(v[i].x, p + i < sq.parts ? fp : 0.f, x);
-      y = __builtin_fmaf(v[i].y, p + i < sq.parts ? fp : 0.f, y);
+      const int64_t at = first + (int64_t)(p + i < sq.parts ? p + i : sq.parts - 1) * a.max_rows;
+      st[i] = *reinterpret_cast<const float2*>(a.ml + at * 4);
+      v[i] = *reinterpret_cast<const f32x4*>(a.acc + at * D + d);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const float m = p + i < sq.parts ? st[i].x : -INFINITY;  // a partition past the last weighs nothing
+      const float top = fmaxf(high, m);
+      const float was = __builtin_amdgcn_exp2f(high - top), is = __builtin_amdgcn_exp2f(m - top);
+      high = top;
+      sum = sum * was + st[i].y * is;
+      x = x * was + v[i] * is;
     }
   }
-  if (d < D) {
-    op[d] = (T)(x * inv);
-    op[d + 1] = (T)(y * inv);
-  }
+  const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+  typedef T T4 __attribute__((ext_vector_type(4)));
+  *reinterpret_cast<T4*>(static_cast<T*>(a.out) + ((int64_t)(sq.first + query) * a.num_heads + h) * D + d) =
+      __builtin_convertvector(x * inv, T4);
 }
 
 template <typename T>
 __global__ void __launch_bounds__(256) pa_tree_join_kernel(const TreeArgs a, const int D, const unsigned join_groups,
-                                                           const int chunks) {
+                                                           const int chunks, const int tile_rows) {
   if (blockIdx.x < join_groups) {
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row < (int64_t)a.num_seqs * a.max_query * a.num_heads) join_row<T>(a, D, row, threadIdx.x & 63);
+    const int lanes = D / 4, rows = 256 / lanes, r = (int)threadIdx.x / lanes;
+    const int64_t row = (int64_t)blockIdx.x * rows + r;
+    if (r < rows && row < (int64_t)a.num_seqs * a.max_query * a.num_heads) join_row<T>(a, D, row, ((int)threadIdx.x - r * lanes) * 4);
     return;
   }
   const unsigned id = blockIdx.x - join_groups;
@@ -81,7 +74,7 @@ __global__ void __launch_bounds__(256) pa_tree_join_kernel(const TreeArgs a, con
   const int head = (int)(id / (unsigned)chunks % (unsigned)a.num_kv_heads);
   const int seq = (int)(id / (unsigned)chunks / (unsigned)a.num_kv_heads);
   const TreeSeq sq = tree_seq(a, seq);
-  if (sq.bad || sq.rows == 0 || chunk * kChunk >= sq.ctx) return;
+  if (sq.bad || sq.rows == 0 || chunk * kChunk >= sq.ctx || tree_whole(sq, tile_rows)) return;
   __shared__ float sm_m[kStatRows], sm_inv[kStatRows];
   const int pos = chunk * kChunk + (int)threadIdx.x * 4;
   f32x4 w = {0, 0, 0, 0};
@@ -109,49 +102,51 @@ __global__ void __launch_bounds__(256) pa_tree_join_kernel(const TreeArgs a, con
       }
     }
   }
-  if (pos >= sq.ctx) return;
-  const int block = a.tables[(int64_t)seq * a.table_width + (pos >> a.block_bits)];
-  if ((unsigned)block >= (unsigned)a.num_blocks) return;
-  // four positions of one block: block sizes are multiples of 8
-  float* wp = a.weights + (((int64_t)block * a.num_kv_heads + head) << a.block_bits) + (pos & ((1 << a.block_bits) - 1));
-  const f32x4 old = *reinterpret_cast<const f32x4*>(wp);
-  const int fresh = sq.ctx - sq.queries;
-#pragma unroll
-  for (int i = 0; i < 4; i++) w[i] = pos + i >= sq.ctx ? old[i] : (pos + i >= fresh ? w[i] : old[i] + w[i]);
-  *reinterpret_cast<f32x4*>(wp) = w;
+  if (pos < sq.ctx) add_weights(a, sq, seq, head, pos, w);
 }
 
 // ---- launch plan ---------------------------------------------------------------------------------
 
 struct TreePlan {
-  int parts, part_len, row_tiles;
+  int parts, part_len, row_tiles, tile_rows;
   int64_t max_rows, logit_stride;
   size_t ml_bytes, acc_bytes, logit_bytes;
   size_t bytes() const { return ml_bytes + acc_bytes + logit_bytes; }
 };
 
 constexpr int kChipCUs = 256;
-constexpr int kPartTokens = 128;   // a partition is a multiple of this
-constexpr int kMaxParts = 64;      // the join gives each a lane
+constexpr int kMaxParts = 64;
+constexpr int kSplitTokens = 1408;
 
-TreePlan tree_plan(int num_seqs, int num_heads, int num_kv_heads, int head_size, int max_ctx, int max_query, bool accumulate) {
+TreePlan tree_plan(int num_seqs, int num_heads, int num_kv_heads, int head_size, int max_ctx, int max_query, bool accumulate,
+                   bool fp32) {
   TreePlan p;
   p.max_rows = (int64_t)max_query * (num_heads / num_kv_heads);
-  const int rows = tree_form(p.max_rows);
+  const int rows = tree_form(p.max_rows, accumulate, fp32);
   p.row_tiles = (int)std::max<int64_t>(1, (p.max_rows + rows - 1) / rows);
   const int64_t groups = std::max<int64_t>(1, (int64_t)num_seqs * num_kv_heads * p.row_tiles);
   // Partitions until there are three workgroups to a CU, none shorter than two steps of every wave.
-  const int64_t want = (3 * kChipCUs + groups - 1) / groups;
-  const int64_t most = std::max<int64_t>(1, (max_ctx + 255) / 256);
+  const int64_t want = tuning_int("PA_TREE_WANT", 2 * kChipCUs) / groups;
+  const int min_part = tuning_int("PA_TREE_MIN_PART", 256);
+  const int64_t most = std::max<int64_t>(1, (max_ctx + min_part - 1) / min_part);
   const int64_t parts = std::max<int64_t>(1, std::min<int64_t>({want, most, (int64_t)kMaxParts}));
-  const int64_t len = (max_ctx + parts - 1) / parts;
-  p.part_len = (int)std::max<int64_t>(kPartTokens, (len + kPartTokens - 1) / kPartTokens * kPartTokens);
+  int64_t len = (max_ctx + parts - 1) / parts;
+  len = std::max<int64_t>(kPartTokens, (len + kPartTokens - 1) / kPartTokens * kPartTokens);
+  if (accumulate) {  // a row's logits and 4 floats behind them, for every row of a workgroup
+    const int64_t room = (tree_logit_floats(head_size, rows / 16) / std::min<int64_t>(rows, p.max_rows) - 4) / kPartTokens * kPartTokens;
+    // A context that does not fit has to go out in parts: shorter ones then, which balance a ragged batch better
+    // (96 sequences of up to 4096 tokens, 8 kv heads: parts of 3072 257 us, of 1408 224, of 768 223).
+    if (len > room) len = std::min<int64_t>(room, kSplitTokens);
+  }
+  p.part_len = (int)len;
   p.parts = (int)std::max<int64_t>(1, ((int64_t)max_ctx + p.part_len - 1) / p.part_len);
+  p.tile_rows = rows;
+  const bool logits = accumulate && (p.parts > 1 || p.row_tiles > 1);
   const size_t cells = (size_t)num_seqs * num_kv_heads * p.parts * p.max_rows;
-  p.ml_bytes = p.parts > 1 || accumulate ? cells * 16 : 0;
+  p.ml_bytes = p.parts > 1 || logits ? cells * 16 : 0;
   p.acc_bytes = p.parts > 1 ? cells * head_size * 4 : 0;
   p.logit_stride = ((int64_t)max_ctx + 31) / 32 * 32;
-  p.logit_bytes = accumulate ? (size_t)num_seqs * num_kv_heads * p.max_rows * p.logit_stride * 4 : 0;
+  p.logit_bytes = logits ? (size_t)num_seqs * num_kv_heads * p.max_rows * p.logit_stride * 4 : 0;
   return p;
 }
 
@@ -188,12 +183,15 @@ int tree_entry(const char* what, void* out, const void* query, const void* key_c
   PA_REQUIRE(max_context_len <= (1 << 30), "%s: max_context_len %d is too large", what, max_context_len);
   PA_REQUIRE(tree_mask == nullptr || mask_stride >= 0, "%s: negative mask stride", what);
   PA_REQUIRE(num_blocks > 0, "%s: the caches have no blocks", what);
-  const TreePlan p = tree_plan(num_seqs, num_heads, num_kv_heads, head_size, max_context_len, max_query_len, accumulate);
+  PA_REQUIRE((int64_t)num_kv_heads * head_size * block_size * elem_size(dtype) <= 0x7fffffff, "%s: a block of a cache exceeds 2 GiB", what);
+  const TreePlan p = tree_plan(num_seqs, num_heads, num_kv_heads, head_size, max_context_len, max_query_len, accumulate,
+                                dtype == PA_DTYPE_F32);
   const int64_t items = (int64_t)num_seqs * num_kv_heads * p.parts;
   const int64_t grid = (items + 7) / 8 * 8 * p.row_tiles;
-  const int64_t join_groups = p.parts > 1 ? ((int64_t)num_seqs * max_query_len * num_heads + 3) / 4 : 0;
+  const int rows_per_group = 256 / (head_size / 4);
+  const int64_t join_groups = p.parts > 1 ? ((int64_t)num_seqs * max_query_len * num_heads + rows_per_group - 1) / rows_per_group : 0;
   const int chunks = (max_context_len + kChunk - 1) / kChunk;
-  const int64_t join_grid = join_groups + (accumulate ? (int64_t)num_seqs * num_kv_heads * chunks : 0);
+  const int64_t join_grid = join_groups + (p.logit_bytes ? (int64_t)num_seqs * num_kv_heads * chunks : 0);
   PA_REQUIRE(grid <= 0x7fffffff && join_grid <= 0x7fffffff && p.max_rows <= 0x7fffffff, "%s: too many rows for one launch", what);
   PA_REQUIRE(p.bytes() == 0 || (workspace && aligned16(workspace) && workspace_bytes >= p.bytes()),
              "%s: workspace of %zu bytes, 16-byte aligned, needed", what, p.bytes());
@@ -211,7 +209,7 @@ int tree_entry(const char* what, void* out, const void* query, const void* key_c
   char* ws = static_cast<char*>(workspace);
   a.ml = reinterpret_cast<float*>(ws);
   a.acc = reinterpret_cast<float*>(ws + p.ml_bytes);
-  a.logits = reinterpret_cast<float*>(ws + p.ml_bytes + p.acc_bytes);
+  a.logits = p.logit_bytes ? reinterpret_cast<float*>(ws + p.ml_bytes + p.acc_bytes) : nullptr;
   a.q_stride = q_stride;
   a.mask_stride = mask_stride;
   a.logit_stride = p.logit_stride;
@@ -231,6 +229,7 @@ int tree_entry(const char* what, void* out, const void* query, const void* key_c
   a.parts = p.parts;
   a.part_len = p.part_len;
   a.row_tiles = p.row_tiles;
+  a.form = p.tile_rows;
   hipStream_t st = static_cast<hipStream_t>(stream);
   int rc;
   switch (dtype) {
@@ -241,9 +240,9 @@ int tree_entry(const char* what, void* out, const void* query, const void* key_c
   if (rc != PA_OK || join_grid == 0) return rc;
   const dim3 jg((unsigned)join_grid), jb(256);
   switch (dtype) {
-    case PA_DTYPE_F32: hipLaunchKernelGGL((pa_tree_join_kernel<float>), jg, jb, 0, st, a, head_size, (unsigned)join_groups, chunks); break;
-    case PA_DTYPE_F16: hipLaunchKernelGGL((pa_tree_join_kernel<_Float16>), jg, jb, 0, st, a, head_size, (unsigned)join_groups, chunks); break;
-    default: hipLaunchKernelGGL((pa_tree_join_kernel<__bf16>), jg, jb, 0, st, a, head_size, (unsigned)join_groups, chunks); break;
+    case PA_DTYPE_F32: hipLaunchKernelGGL((pa_tree_join_kernel<float>), jg, jb, 0, st, a, head_size, (unsigned)join_groups, chunks, p.tile_rows); break;
+    case PA_DTYPE_F16: hipLaunchKernelGGL((pa_tree_join_kernel<_Float16>), jg, jb, 0, st, a, head_size, (unsigned)join_groups, chunks, p.tile_rows); break;
+    default: hipLaunchKernelGGL((pa_tree_join_kernel<__bf16>), jg, jb, 0, st, a, head_size, (unsigned)join_groups, chunks, p.tile_rows); break;
   }
   PA_CHECK_LAUNCH(what);
   return PA_OK;
@@ -253,11 +252,13 @@ int tree_entry(const char* what, void* out, const void* query, const void* key_c
 }  // namespace pa
 
 extern "C" size_t pa_tree_workspace_bytes(int num_seqs, int num_heads, int num_kv_heads, int head_size, int max_context_len,
-                                          int max_query_len, int accumulate) {
+                                          int max_query_len, int accumulate, int dtype) {
   if (num_seqs <= 0 || num_heads <= 0 || num_kv_heads <= 0 || head_size <= 0 || max_context_len <= 0 || max_query_len <= 0 ||
       num_heads % num_kv_heads != 0)
     return 0;
-  return pa::tree_plan(num_seqs, num_heads, num_kv_heads, head_size, max_context_len, max_query_len, accumulate != 0).bytes();
+  return pa::tree_plan(num_seqs, num_heads, num_kv_heads, head_size, max_context_len, max_query_len, accumulate != 0,
+                       dtype == PA_DTYPE_F32)
+      .bytes();
 }
 
 extern "C" int pa_tree_cached_kv_attention(

@@ -22,6 +22,8 @@
 // 2^-20 of the row's largest still has all its bits.
 #pragma once
 
+#include <type_traits>
+
 #include "pa_tree.h"
 
 namespace pa {
@@ -47,7 +49,8 @@ struct F16 {
     for (int i = 0; i < 8; i++) f[i] = (_Float16)p[i];
     return __builtin_bit_cast(u32x4, f);
   }
-  static constexpr uint32_t kOnes = 0x3c003c00u, kInf = 0x7c00u, kSign = 0x8000u;
+  static constexpr uint32_t kOnes = 0x3c003c00u, kExponent = 0x7c007c00u, kLow = 0x04000400u, kSign = 0x80008000u;
+  static constexpr int kToSign = 5;  // from an exponent's lowest bit to the sign's
 };
 
 struct BF16 {
@@ -64,7 +67,8 @@ struct BF16 {
     for (int i = 0; i < 8; i++) f[i] = (__bf16)p[i];
     return __builtin_bit_cast(u32x4, f);
   }
-  static constexpr uint32_t kOnes = 0x3f803f80u, kInf = 0x7f80u, kSign = 0x8000u;
+  static constexpr uint32_t kOnes = 0x3f803f80u, kExponent = 0x7f807f80u, kLow = 0x00800080u, kSign = 0x80008000u;
+  static constexpr int kToSign = 8;
 };
 
 // One 16-byte load holds 4 elements: a product of 16 x 16 x 16 is four instructions, each with one
@@ -82,25 +86,31 @@ struct F32 {
   static __device__ __forceinline__ u32x4 pack(const float* p) {
     return u32x4{__float_as_uint(p[0]), __float_as_uint(p[1]), __float_as_uint(p[2]), __float_as_uint(p[3])};
   }
-  static constexpr uint32_t kOnes = 0x3f800000u, kInf = 0x7f800000u, kSign = 0x80000000u;
+  static constexpr uint32_t kOnes = 0x3f800000u, kExponent = 0x7f800000u, kLow = 0x00800000u, kSign = 0x80000000u;
+  static constexpr int kToSign = 8;
 };
 
-// element i of a vector of kX, as its bits
-template <typename E> __device__ __forceinline__ uint32_t element(u32x4 v, int i) {
-  if (sizeof(typename E::storage) == 4) return v[i];
-  return (v[i >> 1] >> (16 * (i & 1))) & 0xffffu;
+// The elements of one word that are infinite or NaN, by their sign bits: an exponent of all ones carries
+// into the sign's place.  Whole numbers only: compares would need a pair of scalar registers each, and
+// steps that are seldom taken must not weigh on the loop around them.
+template <typename E> __device__ __forceinline__ uint32_t odd_signs(uint32_t w) { return ((w & E::kExponent) + E::kLow) & E::kSign; }
+// of those, the NaN: their other bits, plus all ones, carry into the exponent's lowest place
+template <typename E> __device__ __forceinline__ uint32_t nan_signs(uint32_t w) {
+  const uint32_t rest = ~(E::kExponent | E::kSign);
+  return ((((w & rest) + rest) & E::kLow) << E::kToSign) & odd_signs<E>(w);
+}
+// sign bits to all bits of their elements
+template <typename E> __device__ __forceinline__ uint32_t whole(uint32_t signs) {
+  return sizeof(typename E::storage) == 4 ? (uint32_t)((int32_t)signs >> 31) : (signs >> 15) * 0xffffu;
 }
 
-// `with` in the places (16 or 32 bits) whose bits in v the predicate picks, 0 elsewhere
-template <typename E, typename F> __device__ __forceinline__ u32x4 where(u32x4 v, F pick, u32x4 with) {
+// v with only its first `count` elements (0 .. x) kept
+template <typename E> __device__ __forceinline__ u32x4 first_elements(u32x4 v, int count) {
   u32x4 r;
-  if (sizeof(typename E::storage) == 4) {
 #pragma unroll
-    for (int i = 0; i < 4; i++) r[i] = pick(i, v[i]) ? with[i] : 0u;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-      r[i] = (pick(2 * i, v[i] & 0xffffu) ? with[i] & 0xffffu : 0u) | (pick(2 * i + 1, v[i] >> 16) ? with[i] & 0xffff0000u : 0u);
+  for (int i = 0; i < 4; i++) {
+    if (sizeof(typename E::storage) == 4) r[i] = i < count ? v[i] : 0u;
+    else r[i] = 2 * i + 1 < count ? v[i] : (2 * i < count ? v[i] & 0xffffu : 0u);
   }
   return r;
 }
@@ -110,23 +120,20 @@ template <bool STREAM> __device__ __forceinline__ u32x4 load16(const char* p) {
   return *reinterpret_cast<const u32x4*>(p);
 }
 
-// x elements of a query row from element `at`, whatever its alignment
-template <typename E> __device__ __forceinline__ u32x4 load_query(const typename E::storage* p, bool aligned, int mode) {
-  u32x4 v;
-  if (aligned) {
-    v = *reinterpret_cast<const u32x4*>(p);
-  } else {
-    typename E::frag t;
+// x elements of a query row
+template <typename E> __device__ __forceinline__ u32x4 load_query(const typename E::storage* p, bool aligned) {
+  if (aligned) return *reinterpret_cast<const u32x4*>(p);
+  typename E::frag t;
 #pragma unroll
-    for (int i = 0; i < E::kX; i++) t[i] = p[i];
-    v = __builtin_bit_cast(u32x4, t);
-  }
-  if (mode == 1) {
-#pragma unroll
-    for (int i = 0; i < 4; i++) v[i] ^= sizeof(typename E::storage) == 2 ? 0x80008000u : 0x80000000u;
-  }
-  if (mode == 2) v = u32x4{0, 0, 0, 0};
-  return v;
+  for (int i = 0; i < E::kX; i++) t[i] = p[i];
+  return __builtin_bit_cast(u32x4, t);
+}
+
+// A barrier that orders LDS alone: __syncthreads() would wait for the loads that are on their way, too.
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
 // The workgroup's item.  Workgroups that share a (sequence, partition, head) share an XCD and its L2;
@@ -170,52 +177,110 @@ struct Rows {
   int query[RT], row[RT];
   bool valid[RT];
 
+  // The rows and their queries, as they lie in memory; set() makes them operands once they are there.
   __device__ __forceinline__ void init(const TreeArgs& a, const TreeSeq& sq, int head, int row0, int lane) {
     const int n = lane & 15, g = lane >> 4;
     const bool aligned = ((reinterpret_cast<uintptr_t>(a.q) | (uintptr_t)(a.q_stride * (int64_t)sizeof(T))) & 15u) == 0;
+    const T* qp[RT];
 #pragma unroll
     for (int t = 0; t < RT; t++) {
       row[t] = row0 + t * 16 + n;
       valid[t] = row[t] < sq.rows;
       query[t] = valid[t] ? row[t] / a.group : 0;
       const int hq = valid[t] ? row[t] - query[t] * a.group : 0;
-      const T* qp = static_cast<const T*>(a.q) + (int64_t)(sq.first + query[t]) * a.q_stride + (int64_t)(head * a.group + hq) * D;
-#pragma unroll
-      for (int ks = 0; ks < KS; ks++) {
-        const int chunk = ks * 4 + g;
-        qf[t][ks] = valid[t] && chunk < D / X ? load_query<E>(qp + chunk * X, aligned, a.q_mode) : u32x4{0, 0, 0, 0};
-      }
+      qp[t] = static_cast<const T*>(a.q) + (int64_t)(sq.first + query[t]) * a.q_stride + (int64_t)(head * a.group + hq) * D;
       m[t] = kNoMax;
       lx[t] = 0.f;
       l[t] = f32x4{0, 0, 0, 0};
 #pragma unroll
       for (int j = 0; j < NJ; j++) o[t][j] = f32x4{0, 0, 0, 0};
     }
+    // every lane reads a row that is there and a chunk within it, so that all the loads go out together
+    const auto load = [&](bool whole_chunks) {
+#pragma unroll
+      for (int t = 0; t < RT; t++)
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) qf[t][ks] = load_query<E>(qp[t] + (ks * 4 + g < D / X ? ks * 4 + g : 0) * X, whole_chunks);
+    };
+    if (aligned) load(true);
+    else load(false);
   }
 
-  // Logits to rounded weights, the running maximum and sums kept.  tok: the step's first token.
-  __device__ __forceinline__ u32x4 weigh(const TreeArgs& a, const TreeSeq& sq, int t, const f32x4* s, int tok, int g, bool masked,
-                                         float* logits) {
-    float x[PT];
+  __device__ __forceinline__ void set(const TreeArgs& a, int g) {
+    const uint32_t flip = a.q_mode == 1 ? E::kSign : 0u;  // the scale's sign; a scale of 0 takes q as 0
 #pragma unroll
-    for (int i = 0; i < PT; i++) x[i] = s[i >> 2][i & 3];
-    if (masked) {
-      const int free_end = sq.ctx - sq.queries;
+    for (int t = 0; t < RT; t++)
 #pragma unroll
-      for (int i = 0; i < PT; i++) {
-        const int pos = tok + PT * g + i, d = pos - free_end;
-        bool sees = pos < sq.ctx;
-        if (sees && d >= 0)
-          sees = a.mask == nullptr ? d <= query[t] : a.mask[(int64_t)(sq.first + query[t]) * a.mask_stride + d] != 0;
-        if (!sees) x[i] = -__builtin_inff();
+      for (int ks = 0; ks < KS; ks++) {
+        const bool there = valid[t] & (ks * 4 + g < D / X) & (a.q_mode != 2);
+#pragma unroll
+        for (int i = 0; i < 4; i++) qf[t][ks][i] = there ? qf[t][ks][i] ^ flip : 0u;
+      }
+  }
+
+  // Which of a lane's places of a step the rows see, in a step that ends past what all see: loads first, so that
+  // they are on their way while the logits are made.  tok: the step's first token.
+  struct Seen { uint64_t b[RT]; };
+  __device__ __forceinline__ Seen look(const TreeArgs& a, const TreeSeq& sq, int tok, int g) {
+    Seen v;
+    const int d0 = tok + PT * g - (sq.ctx - sq.queries);  // d0 + i: the drafted position, if not negative
+#pragma unroll
+    for (int t = 0; t < RT; t++) {
+      v.b[t] = 0;
+      if (a.mask == nullptr) continue;
+      const uint8_t* row = a.mask + (int64_t)(sq.first + query[t]) * a.mask_stride;
+      if (a.max_query >= 8) {  // 8 places at once, within the row, then moved to where they belong
+        const int last = a.max_query - 8, from = d0 < 0 ? 0 : (d0 < last ? d0 : last);
+        __builtin_memcpy(&v.b[t], row + from, 8);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 7; i++) v.b[t] |= (uint64_t)(i < sq.queries ? row[i] : 0) << (8 * i);
       }
     }
-    float top = x[0];
+    return v;
+  }
+  // -inf in the logits where a row does not see
+  __device__ __forceinline__ void hide(const TreeArgs& a, const TreeSeq& sq, f32x4 (*s)[NA], const Seen& v, int tok, int g) {
+    const int from = tok + PT * g, d0 = from - (sq.ctx - sq.queries);
+    const int inside = sq.ctx - from;  // places of this lane within the context
+    const uint32_t in_context = inside >= PT ? 0xffffffffu : (inside <= 0 ? 0u : (1u << inside) - 1u);
+    const uint32_t open = d0 >= 0 ? 0u : (d0 <= -PT ? 0xffffffffu : (1u << -d0) - 1u);  // places that all see
 #pragma unroll
-    for (int i = 1; i < PT; i++) top = fmaxf(top, x[i]);
-    top *= a.c;
-    if (__builtin_amdgcn_ballot_w64(top > m[t] + (E::kBias + kMaxSlack)) != 0) {
-      float high = fmaxf(m[t], top - E::kBias);
+    for (int t = 0; t < RT; t++) {
+      uint32_t sees = 0;
+      if (a.mask == nullptr) {
+        const int n = query[t] - d0 + 1;
+        sees = n >= PT ? 0xffffffffu : (n <= 0 ? 0u : (1u << n) - 1u);
+      } else {
+        const int last = a.max_query >= 8 ? a.max_query - 8 : 0, read = d0 < 0 ? 0 : (d0 < last ? d0 : last), by = d0 - read;
+        uint64_t b = by >= 8 || by <= -8 ? 0 : (by >= 0 ? v.b[t] >> (8 * by) : v.b[t] << (-8 * by));
+        b |= b >> 4;  // a truth value to its lowest bit
+        b |= b >> 2;
+        b |= b >> 1;
+        sees = (uint32_t)(((b & 0x0101010101010101ull) * 0x0102040810204080ull) >> 56);  // bit i: byte i's
+      }
+      sees = (sees | open) & in_context;
+#pragma unroll
+      for (int i = 0; i < PT; i++) s[t][i >> 2][i & 3] = (sees >> i) & 1u ? s[t][i >> 2][i & 3] : -__builtin_inff();
+    }
+  }
+
+  // Raises the running maxima where a logit exceeds one by its slack
+  __device__ __forceinline__ void raise(const TreeArgs& a, const f32x4 (*s)[NA]) {
+    float top[RT];
+    bool over = false;
+#pragma unroll
+    for (int t = 0; t < RT; t++) {
+      top[t] = s[t][0][0];
+#pragma unroll
+      for (int i = 1; i < PT; i++) top[t] = fmaxf(top[t], s[t][i >> 2][i & 3]);
+      top[t] *= a.c;
+      over |= top[t] > m[t] + (E::kBias + kMaxSlack);
+    }
+    if (__builtin_amdgcn_ballot_w64(over) == 0) return;
+#pragma unroll
+    for (int t = 0; t < RT; t++) {
+      float high = fmaxf(m[t], top[t] - E::kBias);
       high = fmaxf(high, __shfl_xor(high, 16));
       high = fmaxf(high, __shfl_xor(high, 32));
       const float f = __builtin_amdgcn_exp2f(m[t] - high);
@@ -225,14 +290,15 @@ struct Rows {
 #pragma unroll
       for (int j = 0; j < NJ; j++) o[t][j] *= f;
     }
-    if (logits != nullptr && valid[t]) {
-      float* to = logits + row[t] * a.logit_stride + tok + PT * g;
+  }
+
+  // Logits to rounded weights, and their sum; EXACT: the sum before the rounding too
+  template <bool EXACT>
+  __device__ __forceinline__ u32x4 weigh(const TreeArgs& a, int t, const f32x4* s) {
+    float x[PT];
 #pragma unroll
-      for (int i = 0; i < PT; i += 4) *reinterpret_cast<f32x4*>(to + i) = f32x4{x[i] * a.c, x[i + 1] * a.c, x[i + 2] * a.c, x[i + 3] * a.c};
-    }
-#pragma unroll
-    for (int i = 0; i < PT; i++) x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], a.c, -m[t]));
-    if (logits != nullptr) {
+    for (int i = 0; i < PT; i++) x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i >> 2][i & 3], a.c, -m[t]));
+    if (EXACT) {
 #pragma unroll
       for (int i = 0; i < PT; i++) lx[t] += x[i];
     }
@@ -241,25 +307,34 @@ struct Rows {
     return p;
   }
 
-  // One run of 16 elements of the values in a step that ends past what all rows see.  What lies behind the
-  // context is nobody's and may be anything: it is taken as 0.  A drafted position may hold infinities or
-  // NaN that only the rows that see it must show, and a product with a weight of 0 would hand them to all:
-  // such elements are taken out, and put back where the weight is not 0.
-  __device__ __forceinline__ u32x4 clean(const TreeSeq& sq, u32x4 v, const u32x4* pf, int j, int tok, int g) {
-    v = where<E>(v, [&](int i, uint32_t) { return tok + PT * g + i < sq.ctx; }, v);
-    bool odd = false;
+  // The values of a step that ends past what all rows see.  What lies behind the context is nobody's and may
+  // be anything: it is taken as 0.  A drafted position may hold infinities or NaN that only the rows that see
+  // it must show, and a product with a weight of 0 would hand them to all: such elements are taken out, and put
+  // back where the weight is not 0.
+  __device__ __forceinline__ void clean(const TreeSeq& sq, u32x4* v, const u32x4* pf, int tok, int g) {
+    const int count = sq.ctx - (tok + PT * g);
+    uint32_t odd = 0;
 #pragma unroll
-    for (int i = 0; i < X; i++) odd |= (element<E>(v, i) & E::kInf) == E::kInf;
-    if (__builtin_amdgcn_ballot_w64(odd) != 0) {
-      const u32x4 ones = u32x4{E::kOnes, E::kOnes, E::kOnes, E::kOnes};
+    for (int j = 0; j < NJ; j++) {
+      v[j] = first_elements<E>(v[j], count);
+#pragma unroll
+      for (int i = 0; i < 4; i++) odd |= odd_signs<E>(v[j][i]);
+    }
+    if (__builtin_amdgcn_ballot_w64(odd != 0) == 0) return;
 #pragma unroll 1
-      for (int kind = 0; kind < 3; kind++) {  // +inf, -inf, NaN
-        const float special = kind == 0 ? __builtin_inff() : (kind == 1 ? -__builtin_inff() : __builtin_nanf(""));
-        const u32x4 is = where<E>(v, [&](int, uint32_t b) {
-          if (kind == 0) return b == E::kInf;
-          if (kind == 1) return b == (E::kInf | E::kSign);
-          return (b & (E::kSign - 1u)) > E::kInf;
-        }, ones);
+    for (int kind = 0; kind < 3; kind++) {  // +inf, -inf, NaN
+      const float special = kind == 0 ? __builtin_inff() : (kind == 1 ? -__builtin_inff() : __builtin_nanf(""));
+      const uint32_t nan = kind == 2 ? E::kSign : 0u, flip = kind == 0 ? 0xffffffffu : 0u;
+#pragma unroll
+      for (int j = 0; j < NJ; j++) {
+        u32x4 is;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          uint32_t w = v[j][i];
+          asm volatile("" : "+v"(w));  // made anew each time: what could be kept for the next would fill the registers
+          const uint32_t n = nan_signs<E>(w);
+          is[i] = E::kOnes & whole<E>((n & nan) | (odd_signs<E>(w) & ~n & (w ^ flip) & ~nan));
+        }
 #pragma unroll
         for (int t = 0; t < RT; t++) {
           const f32x4 hit = E::mma(is, pf[t], f32x4{0, 0, 0, 0});
@@ -267,9 +342,15 @@ struct Rows {
           for (int i = 0; i < 4; i++) o[t][j][i] += hit[i] > 0.f ? special : 0.f;
         }
       }
-      v = where<E>(v, [&](int, uint32_t b) { return (b & E::kInf) != E::kInf; }, v);
     }
-    return v;
+#pragma unroll
+    for (int j = 0; j < NJ; j++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        uint32_t w = v[j][i];
+        asm volatile("" : "+v"(w));
+        v[j][i] = w & ~whole<E>(odd_signs<E>(w));
+      }
   }
 
   __device__ __forceinline__ void finish_exact() {
@@ -295,7 +376,7 @@ __device__ __forceinline__ void store_row(const TreeArgs& a, const TreeSeq& sq, 
     typedef T T4 __attribute__((ext_vector_type(4)));
     *reinterpret_cast<T4*>(op) = __builtin_convertvector(v * inv, T4);
   }
-  if ((sq.parts > 1 || a.weights != nullptr) && d == 0)
+  if ((sq.parts > 1 || a.logits != nullptr) && d == 0)
     *reinterpret_cast<f32x4*>(a.ml + tree_row(a, it.seq, it.head, it.part, row) * 4) = f32x4{mx, sum, exact, 0.f};
 }
 
@@ -304,7 +385,11 @@ __device__ __forceinline__ void store_row(const TreeArgs& a, const TreeSeq& sq, 
 // All 4 waves have the same RT tiles of rows; they take turns at the steps of the context and add up
 // through LDS.  A wave holds the keys and the values of one step: the next keys are on their way while
 // the weights are made, the next values while the next logits are.
-template <typename E, int D, int B, int RT>
+// ACC: the weight cache is added to.  A partition's logits stay in LDS (which bounds its length).  Where it is
+// the sequence's only one the weights are made of them here; else they go out together at the end, for the
+// kernel that joins partitions.  Written out step by step, with the loop's reads, they cost three times as much
+// (96 sequences of up to 4096 tokens, 4 query heads to a kv head: 48 us of 247, for 31 MB).
+template <typename E, int D, int B, int RT, bool ACC>
 __global__ void __launch_bounds__(256, (RT == 1 ? 3 : 2)) pa_tree_few_kernel(const TreeArgs a) {
   typedef typename E::storage T;
   typedef Rows<E, D, RT> R;
@@ -320,17 +405,19 @@ __global__ void __launch_bounds__(256, (RT == 1 ? 3 : 2)) pa_tree_few_kernel(con
   const int row0 = it.tile * ROWS;
   if (row0 >= sq.rows || it.part >= sq.parts) return;
   const int n = lane & 15, g = lane >> 4;
-  const int p0 = it.part * a.part_len;
-  const int p1 = it.part == sq.parts - 1 ? sq.ctx : p0 + a.part_len;
+  const int p0 = it.part * sq.part_len;
+  const int p1 = it.part == sq.parts - 1 ? sq.ctx : p0 + sq.part_len;
   const int steps = (p1 - p0 + TS - 1) / TS;
-  float* logits = a.weights == nullptr ? nullptr : a.logits + ((int64_t)it.seq * a.num_kv_heads + it.head) * a.max_rows * a.logit_stride;
-
+  const int open = sq.ctx - sq.queries - p0, open_steps = open < 0 ? 0 : (open / TS < steps ? open / TS : steps);  // seen by all rows
   R r;
-  r.init(a, sq, it.head, row0, lane);
+  __shared__ float sm_m[WK][ROWS], sm_l[WK][ROWS], sm_x[WK][ROWS];
+  constexpr int ST = D + 4;  // rows of LDS start 4 banks apart
+  __shared__ __attribute__((aligned(16))) float sm[ACC ? tree_logit_floats(D, RT) : WK * ROWS * ST];
+  const int logit_row = sq.part_len + 4;
 
   const int32_t* table = a.tables + (int64_t)it.seq * a.table_width;
   const int last_entry = (sq.ctx - 1) / B;
-  const int64_t block_bytes = (int64_t)a.num_kv_heads * D * B * (int)sizeof(T);
+  const uint32_t block_bytes = (uint32_t)a.num_kv_heads * (uint32_t)(D * B * (int)sizeof(T));  // under 2^32: checked on the host
   const char* kc = a.kc + (int64_t)it.head * D * B * (int)sizeof(T);
   const char* vc = a.vc + (int64_t)it.head * D * B * (int)sizeof(T);
   // the first of this lane's tokens of a step: on the key side (row m = n) and on the value side
@@ -354,7 +441,7 @@ __global__ void __launch_bounds__(256, (RT == 1 ? 3 : 2)) pa_tree_few_kernel(con
   };
   u32x4 kf[NA][KS], vf[NJ];
   const auto load_k = [&](int b, int step) {
-    const char* base = kc + (int64_t)checked(b) * block_bytes + (((p0 + step * TS + ktok) & (B - 1)) + g * B) * 16;
+    const char* base = kc + (uint64_t)(uint32_t)checked(b) * block_bytes + (((p0 + step * TS + ktok) & (B - 1)) + g * B) * 16;
 #pragma unroll
     for (int i = 0; i < NA; i++)
 #pragma unroll
@@ -364,20 +451,31 @@ __global__ void __launch_bounds__(256, (RT == 1 ? 3 : 2)) pa_tree_few_kernel(con
       }
   };
   const auto load_v = [&](int b, int step) {
-    const char* base = vc + (int64_t)checked(b) * block_bytes + (((p0 + step * TS + vtok) & (B - 1)) + n * B) * (int)sizeof(T);
+    const char* base = vc + (uint64_t)(uint32_t)checked(b) * block_bytes + (((p0 + step * TS + vtok) & (B - 1)) + n * B) * (int)sizeof(T);
 #pragma unroll
     for (int j = 0; j < NJ; j++) vf[j] = load16<true>(base + j * 16 * B * (int)sizeof(T));
   };
 
   int step = wk;
-  if (step < steps) {
-    Ids next = load_ids(step);
-    load_k(next.k, step);
-    load_v(next.v, step);
-    next = load_ids(step + WK < steps ? step + WK : step);
-    for (; step < steps; step += WK) {
-      const bool more = step + WK < steps;
+  if (step >= steps) {
+    r.init(a, sq, it.head, row0, lane);
+  } else {
+    const Ids now = load_ids(step);
+    Ids next = load_ids(step + WK < steps ? step + WK : step);
+    r.init(a, sq, it.head, row0, lane);
+    __builtin_amdgcn_sched_barrier(0);  // in this order, as in the loop: a wait for them must not wait for the blocks
+    load_k(now.k, step);
+    load_v(now.v, step);
+    __builtin_amdgcn_sched_barrier(0);
+    r.set(a, g);
+    // INNER: a step that all rows see, with another behind it.  Its loads are under no condition: a wait can
+    // count on what was issued after the load that it is for only where that is certain.
+    const auto turn = [&](auto inner) {
+      constexpr bool kInner = decltype(inner)::value;
+      const bool more = kInner || step + WK < steps, masked = !kInner && step >= open_steps;
       const int tok = p0 + step * TS;
+      typename R::Seen seen;
+      if (masked) seen = r.look(a, sq, tok, g);
       f32x4 s[RT][NA];
 #pragma unroll
       for (int t = 0; t < RT; t++)
@@ -389,50 +487,93 @@ __global__ void __launch_bounds__(256, (RT == 1 ? 3 : 2)) pa_tree_few_kernel(con
         }
       // the table entries two steps ahead go out before the next keys: waiting for them waits for nothing else
       const Ids after = load_ids(step + 2 * WK < steps ? step + 2 * WK : step);
+      __builtin_amdgcn_sched_barrier(0);  // the loads where they stand: earlier, they would take registers twice
       if (more) load_k(next.k, step + WK);
-      const bool masked = tok + TS > sq.ctx - sq.queries;
+      __builtin_amdgcn_sched_barrier(0);
+      if (masked) r.hide(a, sq, s, seen, tok, g);
+      r.raise(a, s);
       u32x4 pf[RT];
 #pragma unroll
-      for (int t = 0; t < RT; t++) pf[t] = r.weigh(a, sq, t, s[t], tok, g, masked, logits);
-      if (masked) {
+      for (int t = 0; t < RT; t++) {
+        if (ACC) {
+          if (r.valid[t]) {
 #pragma unroll
-        for (int j = 0; j < NJ; j++) vf[j] = r.clean(sq, vf[j], pf, j, tok, g);
+            for (int i = 0; i < NA; i++)
+              *reinterpret_cast<f32x4*>(sm + (t * 16 + n) * logit_row + step * TS + vtok + 4 * i) = s[t][i] * a.c;
+          }
+        }
+        pf[t] = r.template weigh<ACC>(a, t, s[t]);
       }
+      if (masked) r.clean(sq, vf, pf, tok, g);
 #pragma unroll
       for (int t = 0; t < RT; t++)
 #pragma unroll
         for (int j = 0; j < NJ; j++) r.o[t][j] = E::mma(vf[j], pf[t], r.o[t][j]);
+      __builtin_amdgcn_sched_barrier(0);
       if (more) load_v(next.v, step + WK);
+      __builtin_amdgcn_sched_barrier(0);
       next = after;
-    }
+    };
+    for (; step < open_steps && step + WK < steps; step += WK) turn(std::true_type{});
+    for (; step < steps; step += WK) turn(std::false_type{});
   }
   // a block number outside the cache: the rows must not pass for a result
   const bool any_bad = __builtin_amdgcn_ballot_w64(bad_block) != 0;
-  r.finish_exact();
+  if (ACC) r.finish_exact();
 
   // the waves' shares of a row: their maxima first, then the sums at the common scale
-  constexpr int ST = D + 4;  // rows of LDS start 4 banks apart
-  __shared__ float sm_m[WK][ROWS], sm_l[WK][ROWS], sm_x[WK][ROWS];
-  __shared__ __attribute__((aligned(16))) float sm_o[WK][ROWS][ST];
   if (g == 0) {
 #pragma unroll
     for (int t = 0; t < RT; t++) sm_m[wk][t * 16 + n] = r.m[t];
   }
   __syncthreads();
+  float scale[RT];
 #pragma unroll
   for (int t = 0; t < RT; t++) {
     const int row = t * 16 + n;
     float high = sm_m[0][row];
 #pragma unroll
     for (int w = 1; w < WK; w++) high = fmaxf(high, sm_m[w][row]);
-    const float f = any_bad ? __builtin_nanf("") : __builtin_amdgcn_exp2f(r.m[t] - high);
+    scale[t] = any_bad ? __builtin_nanf("") : __builtin_amdgcn_exp2f(r.m[t] - high);
     if (g == 0) {
-      sm_l[wk][row] = r.l[t][0] * f;
-      sm_x[wk][row] = r.lx[t] * f;
+      sm_l[wk][row] = r.l[t][0] * scale[t];
+      sm_x[wk][row] = r.lx[t] * scale[t];
     }
-#pragma unroll
-    for (int j = 0; j < NJ; j++) *reinterpret_cast<f32x4*>(&sm_o[wk][row][16 * j + 4 * g]) = r.o[t][j] * f;
   }
+  if (ACC) {
+    __syncthreads();
+    const int rows = sq.rows - row0 < ROWS ? sq.rows - row0 : ROWS;
+    if (tree_whole(sq, ROWS)) {
+      for (int pos = tid * 4; pos < sq.ctx; pos += 1024) {
+        f32x4 w = {0, 0, 0, 0};
+        for (int row = 0; row < rows; row++) {
+          float high = sm_m[0][row], sum = sm_x[0][row];
+#pragma unroll
+          for (int k = 1; k < WK; k++) {
+            high = fmaxf(high, sm_m[k][row]);
+            sum += sm_x[k][row];
+          }
+          const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+          const f32x4 x = *reinterpret_cast<const f32x4*>(sm + row * logit_row + pos);
+#pragma unroll
+          for (int i = 0; i < 4; i++) w[i] = __builtin_fmaf(__builtin_amdgcn_exp2f(x[i] - high), inv, w[i]);
+        }
+        add_weights(a, sq, it.seq, it.head, pos, w);
+      }
+    } else {
+      float* to = a.logits + (((int64_t)it.seq * a.num_kv_heads + it.head) * a.max_rows + row0) * a.logit_stride + p0;
+      const int len = (p1 - p0 + TS - 1) / TS * TS;
+      for (int row = 0; row < rows; row++)
+        for (int pos = tid * 4; pos < len; pos += 1024)
+          *reinterpret_cast<f32x4*>(to + row * a.logit_stride + pos) = *reinterpret_cast<const f32x4*>(sm + row * logit_row + pos);
+    }
+    __syncthreads();
+  }
+  float (*sm_o)[ROWS][ST] = reinterpret_cast<float (*)[ROWS][ST]>(sm);
+#pragma unroll
+  for (int t = 0; t < RT; t++)
+#pragma unroll
+    for (int j = 0; j < NJ; j++) *reinterpret_cast<f32x4*>(&sm_o[wk][t * 16 + n][16 * j + 4 * g]) = r.o[t][j] * scale[t];
   __syncthreads();
   for (int i = tid; i < ROWS * (D / 4); i += 256) {
     const int row = i / (D / 4), d = (i - row * (D / 4)) * 4;
@@ -454,16 +595,15 @@ __global__ void __launch_bounds__(256, (RT == 1 ? 3 : 2)) pa_tree_few_kernel(con
 //
 // NW waves of RT tiles each.  A step's operands are KS x NA + D / 16 pieces of 1 KiB, in LDS exactly as the
 // products take them (a lane's 16 bytes at 16 * lane: no bank conflicts); wave w fetches pieces w, w + NW, ...
-// from the caches at the addresses that the few-rows kernel would use.  Two buffers: while step i is
-// consumed, the pieces of i + 1 are in registers or on their way, those of i + 2 are on their way; one
-// barrier a step.
+// from the caches at the addresses that the few-rows kernel would use.  Two buffers of each kind, filled from
+// registers that were loaded two turns before; one barrier a step.
 template <typename E, int D, int RT, int NW>
 __global__ void __launch_bounds__(NW * 64, 2) pa_tree_many_kernel(const TreeArgs a) {
   typedef typename E::storage T;
   typedef Rows<E, D, RT> R;
   constexpr int X = R::X, TS = R::TS, KS = R::KS, NA = R::NA, NJ = R::NJ, PT = R::PT, ROWS = 16 * RT * NW;
-  constexpr int PIECES = NA * KS + NJ, F = (PIECES + NW - 1) / NW;
-  __shared__ __attribute__((aligned(16))) u32x4 sm[2][PIECES * 64];
+  constexpr int NK = NA * KS, FK = (NK + NW - 1) / NW, FV = (NJ + NW - 1) / NW;
+  __shared__ __attribute__((aligned(16))) u32x4 sm_k[2][NK * 64], sm_v[2][NJ * 64];
   __shared__ int sm_bad;
   const Item it = tree_item(a);
   if (!it.exists) return;
@@ -477,19 +617,18 @@ __global__ void __launch_bounds__(NW * 64, 2) pa_tree_many_kernel(const TreeArgs
   if (row0 >= sq.rows || it.part >= sq.parts) return;
   const int n = lane & 15, g = lane >> 4;
   const int bits = a.block_bits, B = 1 << bits;
-  const int p0 = it.part * a.part_len;
-  const int p1 = it.part == sq.parts - 1 ? sq.ctx : p0 + a.part_len;
+  const int p0 = it.part * sq.part_len;
+  const int p1 = it.part == sq.parts - 1 ? sq.ctx : p0 + sq.part_len;
   const int steps = (p1 - p0 + TS - 1) / TS;
-  float* logits = a.weights == nullptr ? nullptr : a.logits + ((int64_t)it.seq * a.num_kv_heads + it.head) * a.max_rows * a.logit_stride;
+  const int open = sq.ctx - sq.queries - p0, open_steps = open < 0 ? 0 : (open / TS < steps ? open / TS : steps);  // seen by all rows
   const bool has_rows = row0 + wave * 16 * RT < sq.rows;
   if (tid == 0) sm_bad = 0;
 
   R r;
-  r.init(a, sq, it.head, row0 + wave * 16 * RT, lane);
 
   const int32_t* table = a.tables + (int64_t)it.seq * a.table_width;
   const int last_entry = (sq.ctx - 1) >> bits;
-  const int64_t block_bytes = (int64_t)a.num_kv_heads * D * B * (int)sizeof(T);
+  const uint32_t block_bytes = (uint32_t)a.num_kv_heads * (uint32_t)(D * B * (int)sizeof(T));  // under 2^32: checked on the host
   const char* kc = a.kc + (int64_t)it.head * D * B * (int)sizeof(T);
   const char* vc = a.vc + (int64_t)it.head * D * B * (int)sizeof(T);
   const int ktok = TS == 32 ? 8 * (n >> 2) + (n & 3) : n;
@@ -510,107 +649,164 @@ __global__ void __launch_bounds__(NW * 64, 2) pa_tree_many_kernel(const TreeArgs
     bad_block |= !ok;
     return ok ? b : 0;
   };
-  const auto fetch = [&](u32x4* v, Ids ids, int step) {
-    const int tok = p0 + step * TS;
-    const char* kb = kc + (int64_t)checked(ids.k) * block_bytes + (((tok + ktok) & (B - 1)) + g * B) * 16;
-    const char* vb = vc + (int64_t)checked(ids.v) * block_bytes + (((tok + vtok) & (B - 1)) + n * B) * (int)sizeof(T);
+  // this wave's pieces; a wave beyond their number fetches the last again
+  int k_at[FK], v_at[FV];
+  bool k_in[FK];  // whether this lane's chunk is within the head
+  const auto k_piece = [&](int f) { return wave + f * NW < NK ? wave + f * NW : NK - 1; };
+  const auto v_piece = [&](int f) { return wave + f * NW < NJ ? wave + f * NW : NJ - 1; };
 #pragma unroll
-    for (int f = 0; f < F; f++) {
-      const int piece = wave + f * NW;  // the same for the whole wave
-      v[f] = u32x4{0, 0, 0, 0};
-      if (piece < NA * KS) {
-        const int i = piece / KS, ks = piece - i * KS;
-        if (KS * 4 * X == D || ks * 4 + g < D / X) v[f] = load16<false>(kb + (i * 4 + ks * 4 * B) * 16);
-      } else if (piece < PIECES) {
-        v[f] = load16<false>(vb + (piece - NA * KS) * 16 * B * (int)sizeof(T));
-      }
-    }
-  };
-  const auto put = [&](const u32x4* v, int buffer) {
+  for (int f = 0; f < FK; f++) {
+    const int i = k_piece(f) / KS, ks = k_piece(f) - i * KS;
+    k_in[f] = ks * 4 + g < D / X;
+    k_at[f] = k_in[f] ? (i * 4 + ks * 4 * B) * 16 : 0;
+  }
 #pragma unroll
-    for (int f = 0; f < F; f++)
-      if (wave + f * NW < PIECES) sm[buffer][(wave + f * NW) * 64 + lane] = v[f];
+  for (int f = 0; f < FV; f++) v_at[f] = v_piece(f) * 16 * B * (int)sizeof(T);
+  const auto fetch_k = [&](u32x4* v, int id, int step) {
+    const char* kb = kc + (uint64_t)(uint32_t)checked(id) * block_bytes + (((p0 + step * TS + ktok) & (B - 1)) + g * B) * 16;
+#pragma unroll
+    for (int f = 0; f < FK; f++) v[f] = load16<false>(kb + k_at[f]);
   };
-  const auto consume = [&](int step, const u32x4* buf) {
-    if (!has_rows) return;
-    const int tok = p0 + step * TS;
-    f32x4 s[RT][NA];
+  const auto fetch_v = [&](u32x4* v, int id, int step) {
+    const char* vb = vc + (uint64_t)(uint32_t)checked(id) * block_bytes + (((p0 + step * TS + vtok) & (B - 1)) + n * B) * (int)sizeof(T);
+#pragma unroll
+    for (int f = 0; f < FV; f++) v[f] = load16<false>(vb + v_at[f]);
+  };
+  const auto put_k = [&](const u32x4* v, u32x4* buf) {
+#pragma unroll
+    for (int f = 0; f < FK; f++) buf[k_piece(f) * 64 + lane] = KS * 4 * X == D || k_in[f] ? v[f] : u32x4{0, 0, 0, 0};
+  };
+  const auto put_v = [&](const u32x4* v, u32x4* buf) {
+#pragma unroll
+    for (int f = 0; f < FV; f++) buf[v_piece(f) * 64 + lane] = v[f];
+  };
+  const auto take = [&](u32x4 (*k)[KS], const u32x4* buf) {
+#pragma unroll
+    for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+      for (int i = 0; i < NA; i++) k[i][ks] = buf[(i * KS + ks) * 64 + lane];
+  };
+  const auto multiply = [&](f32x4 (*s)[NA], const u32x4 (*k)[KS]) {
 #pragma unroll
     for (int t = 0; t < RT; t++)
 #pragma unroll
       for (int i = 0; i < NA; i++) s[t][i] = f32x4{0, 0, 0, 0};
 #pragma unroll
-    for (int i = 0; i < NA; i++)
+    for (int ks = 0; ks < KS; ks++)
 #pragma unroll
-      for (int ks = 0; ks < KS; ks++) {
-        const u32x4 k = buf[(i * KS + ks) * 64 + lane];
+      for (int i = 0; i < NA; i++)
 #pragma unroll
-        for (int t = 0; t < RT; t++) s[t][i] = E::mma(k, r.qf[t][ks], s[t][i]);
-      }
-    const bool masked = tok + TS > sq.ctx - sq.queries;
-    u32x4 pf[RT];
-#pragma unroll
-    for (int t = 0; t < RT; t++) pf[t] = r.weigh(a, sq, t, s[t], tok, g, masked, logits);
-#pragma unroll
-    for (int j = 0; j < NJ; j++) {
-      u32x4 v = buf[(NA * KS + j) * 64 + lane];
-      if (masked) v = r.clean(sq, v, pf, j, tok, g);
-#pragma unroll
-      for (int t = 0; t < RT; t++) r.o[t][j] = E::mma(v, pf[t], r.o[t][j]);
-    }
+        for (int t = 0; t < RT; t++) s[t][i] = E::mma(k[i][ks], r.qf[t][ks], s[t][i]);
   };
 
-  // step i's pieces pass through held[i & 1]; a step past the last is the last again
+  // A step past the last is the last again.  Keys run one step ahead of values: when step i's turn comes its
+  // logits are there, and the products of step i + 1's keys have no part in what is made of them, so the
+  // matrix and the vector units work side by side in every wave.
   const auto clamp = [&](int step) { return step < steps ? step : steps - 1; };
-  u32x4 held[2][F];
-  Ids ids = load_ids(0);
-  fetch(held[0], ids, 0);
-  ids = load_ids(clamp(1));
-  Ids after = load_ids(clamp(2));
-  fetch(held[1], ids, clamp(1));
-  put(held[0], 0);
+  u32x4 k_held[2][FK], v_held[2][FV];  // step i's pieces pass through set i % 2; no copies, which would wait for the loads
+  f32x4 s[RT][NA];
+  {
+    const Ids i0 = load_ids(0), i1 = load_ids(clamp(1)), i2 = load_ids(clamp(2));
+    r.init(a, sq, it.head, row0 + wave * 16 * RT, lane);
+    __builtin_amdgcn_sched_barrier(0);
+    fetch_k(k_held[0], i0.k, 0);
+    fetch_k(k_held[1], i1.k, clamp(1));
+    fetch_v(v_held[0], i0.v, 0);
+    fetch_v(v_held[1], i1.v, clamp(1));
+    r.set(a, g);
+    put_k(k_held[0], sm_k[0]);
+    fetch_k(k_held[0], i2.k, clamp(2));
+    put_k(k_held[1], sm_k[1]);
+    put_v(v_held[0], sm_v[0]);
+  }
   __syncthreads();
-  const auto turn = [&](int step, int parity) {
-    ids = after;
-    after = load_ids(clamp(step + 3));
-    fetch(held[parity], ids, clamp(step + 2));
-    consume(step, sm[parity]);
-    put(held[1 - parity], 1 - parity);
-    __syncthreads();
+  {
+    u32x4 k[NA][KS];
+    take(k, sm_k[0]);
+    multiply(s, k);
+  }
+  int next_k = load_ids(clamp(3)).k, next_v = load_ids(clamp(2)).v;
+  const auto turn = [&](auto masked, auto odd, int step) {
+    constexpr bool kMasked = decltype(masked)::value;
+    constexpr int kOdd = decltype(odd)::value;  // step % 2
+    const int id_k = next_k, id_v = next_v;
+    const int tok = p0 + step * TS;
+    typename R::Seen seen;
+    if (kMasked) seen = r.look(a, sq, tok, g);
+    next_k = load_ids(clamp(step + 4)).k;
+    next_v = load_ids(clamp(step + 3)).v;
+    fetch_k(k_held[1 - kOdd], id_k, clamp(step + 3));
+    fetch_v(v_held[kOdd], id_v, clamp(step + 2));
+    if (has_rows) {
+      u32x4 k[NA][KS], v[NJ];
+      take(k, sm_k[1 - kOdd]);  // on their way while the maxima are looked at
+      __builtin_amdgcn_sched_barrier(0);
+      if (kMasked) r.hide(a, sq, s, seen, tok, g);
+      r.raise(a, s);
+      f32x4 ahead[RT][NA];
+      multiply(ahead, k);
+#pragma unroll
+      for (int j = 0; j < NJ; j++) v[j] = sm_v[kOdd][j * 64 + lane];
+      u32x4 pf[RT];
+#pragma unroll
+      for (int t = 0; t < RT; t++) pf[t] = r.template weigh<false>(a, t, s[t]);
+      if (kMasked) r.clean(sq, v, pf, tok, g);
+#pragma unroll
+      for (int j = 0; j < NJ; j++)
+#pragma unroll
+        for (int t = 0; t < RT; t++) r.o[t][j] = E::mma(v[j], pf[t], r.o[t][j]);
+#pragma unroll
+      for (int t = 0; t < RT; t++)
+#pragma unroll
+        for (int i = 0; i < NA; i++) s[t][i] = ahead[t][i];
+    }
+    put_k(k_held[kOdd], sm_k[kOdd]);
+    put_v(v_held[1 - kOdd], sm_v[1 - kOdd]);
+    lds_barrier();
   };
-  for (int step = 0; step < steps; step += 2) {
-    turn(step, 0);
-    if (step + 1 < steps) turn(step + 1, 1);
+  int step = 0;
+  constexpr std::integral_constant<int, 0> even{};
+  constexpr std::integral_constant<int, 1> odd{};
+  for (; step + 1 < open_steps; step += 2) {
+    turn(std::false_type{}, even, step);
+    turn(std::false_type{}, odd, step + 1);
+  }
+  for (; step < steps; step += 2) {  // an open step among them is looked at like the others
+    turn(std::true_type{}, even, step);
+    if (step + 1 < steps) turn(std::true_type{}, odd, step + 1);
   }
   if (bad_block) sm_bad = 1;
   __syncthreads();
   const bool any_bad = sm_bad != 0;
-  r.finish_exact();
 #pragma unroll
   for (int t = 0; t < RT; t++)
     if (r.valid[t]) {
-      const float sum = any_bad ? __builtin_nanf("") : r.l[t][0], exact = any_bad ? __builtin_nanf("") : r.lx[t];
+      const float sum = any_bad ? __builtin_nanf("") : r.l[t][0];
 #pragma unroll
-      for (int j = 0; j < NJ; j++) store_row<E, D>(a, sq, it, r.row[t], 16 * j + 4 * g, r.o[t][j], r.m[t], sum, exact);
+      for (int j = 0; j < NJ; j++) store_row<E, D>(a, sq, it, r.row[t], 16 * j + 4 * g, r.o[t][j], r.m[t], sum, 0.f);
     }
+}
+
+template <typename E, int D, int B>
+static void tree_few(const TreeArgs& a, int form, unsigned grid, hipStream_t st) {
+  if (a.weights != nullptr) {
+    if (form == kTreeFew16) hipLaunchKernelGGL((pa_tree_few_kernel<E, D, B, 1, true>), dim3(grid), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((pa_tree_few_kernel<E, D, B, 2, true>), dim3(grid), dim3(256), 0, st, a);
+  } else {
+    if (form == kTreeFew16) hipLaunchKernelGGL((pa_tree_few_kernel<E, D, B, 1, false>), dim3(grid), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((pa_tree_few_kernel<E, D, B, 2, false>), dim3(grid), dim3(256), 0, st, a);
+  }
 }
 
 template <typename E, int D>
 static void tree_pick_form(const TreeArgs& a, unsigned grid, hipStream_t st) {
-  const int form = tree_form(a.max_rows);
+  const int form = a.form;
   if (form == kTreeMany64) hipLaunchKernelGGL((pa_tree_many_kernel<E, D, 1, 4>), dim3(grid), dim3(256), 0, st, a);
-  else if (form == kTreeMany128) hipLaunchKernelGGL((pa_tree_many_kernel<E, D, 2, 4>), dim3(grid), dim3(256), 0, st, a);
-  else if (form == kTreeMany256) hipLaunchKernelGGL((pa_tree_many_kernel<E, D, 2, 8>), dim3(grid), dim3(512), 0, st, a);
+  else if (form == kTreeMany128) hipLaunchKernelGGL((pa_tree_many_kernel<E, D, (E::kX == 8 ? 2 : 1), 4>), dim3(grid), dim3(256), 0, st, a);
   else {
-#define PA_TREE_FEW(B)                                                                                                   \
-  do {                                                                                                                   \
-    if (form == kTreeFew16) hipLaunchKernelGGL((pa_tree_few_kernel<E, D, B, 1>), dim3(grid), dim3(256), 0, st, a);       \
-    else hipLaunchKernelGGL((pa_tree_few_kernel<E, D, B, 2>), dim3(grid), dim3(256), 0, st, a);                          \
-  } while (0)
-    if (a.block_bits == 3) PA_TREE_FEW(8);
-    else if (a.block_bits == 4) PA_TREE_FEW(16);
-    else PA_TREE_FEW(32);
-#undef PA_TREE_FEW
+    if (a.block_bits == 3) tree_few<E, D, 8>(a, form, grid, st);
+    else if (a.block_bits == 4) tree_few<E, D, 16>(a, form, grid, st);
+    else tree_few<E, D, 32>(a, form, grid, st);
   }
 }
 
