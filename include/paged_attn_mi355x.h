@@ -370,8 +370,7 @@ int pa_gather_cached_kv(
  * block sizes 8, 16, 32; all pa_dtype values.  workspace: pa_evict_workspace_bytes
  * of device memory, 16-byte aligned, contents irrelevant.
  */
-size_t pa_evict_workspace_bytes(int num_seqs, int num_kv_heads,
-                                int max_context_len);
+size_t pa_evict_workspace_bytes(int num_seqs, int num_kv_heads);
 
 int pa_evict_cached_kv(
     void* key_cache, void* value_cache, float* weight_cache,

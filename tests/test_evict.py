@@ -110,7 +110,7 @@ def test_ties_and_special_weights(pkg, weights, recent):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("n", [8191, 8192, 8193, 20000])
+@pytest.mark.parametrize("n", [8191, 8192, 8193, 16383, 16384, 16385, 20000, 40000])
 def test_long_contexts(pkg, n):
     """About as many positions as the selection holds in LDS, and more."""
     run(pkg, Case([n, 5000], n // 3, n // 10, heads=1))
@@ -205,8 +205,9 @@ def test_c_entry_refuses_without_a_gpu(pkg):
     assert call(mc=65) == c.PA_ERR_INVALID_ARGUMENT and "cannot hold" in c.last_error()
     assert call(ws=None) == c.PA_ERR_INVALID_ARGUMENT and "workspace" in c.last_error()
     assert call(wb=10) == c.PA_ERR_INVALID_ARGUMENT and "workspace" in c.last_error()
+    assert call(nb=1 << 28) == c.PA_ERR_INVALID_ARGUMENT and "slots" in c.last_error()
     assert call(S=0) == c.PA_OK and call(H=0) == c.PA_OK
-    assert c.lib.pa_evict_workspace_bytes(2, 2, 64) > 0 and c.lib.pa_evict_workspace_bytes(0, 2, 64) == 0
+    assert c.lib.pa_evict_workspace_bytes(2, 2) > 0 and c.lib.pa_evict_workspace_bytes(0, 2) == 0
 
 
 def test_module_refuses_cpu_tensors(pkg):

@@ -114,7 +114,7 @@ def _load() -> ctypes.CDLL:
     lib.pa_rotary_embedding_neox_reshape_and_cache.argtypes = [
         vp, vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i64, i64, i64, i32, vp]
     lib.pa_rotary_embedding_neox_reshape_and_cache.restype = i32
-    lib.pa_evict_workspace_bytes.argtypes = [i32, i32, i32]
+    lib.pa_evict_workspace_bytes.argtypes = [i32, i32]
     lib.pa_evict_workspace_bytes.restype = ctypes.c_size_t
     lib.pa_evict_cached_kv.argtypes = [vp] * 6 + [i32] * 10 + [vp, ctypes.c_size_t, vp]
     lib.pa_evict_cached_kv.restype = i32

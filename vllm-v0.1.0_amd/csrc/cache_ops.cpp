@@ -225,7 +225,7 @@ void evict_cached_kv(const torch::Tensor& key_cache,      // [num_blocks, num_kv
                   seqs <= INT32_MAX && dim <= INT32_MAX && block_tables.size(1) <= INT32_MAX && num_recent >= 0 && num_recent <= INT32_MAX,
               what, ": size out of range");
   PA_DEVICE_GUARD(key_cache);
-  const size_t bytes = pa_evict_workspace_bytes(static_cast<int>(seqs), static_cast<int>(heads), static_cast<int>(max_context_len));
+  const size_t bytes = pa_evict_workspace_bytes(static_cast<int>(seqs), static_cast<int>(heads));
   const torch::Tensor ws = torch::empty({static_cast<int64_t>(bytes)}, key_cache.options().dtype(torch::kUInt8));
   check_status(pa_evict_cached_kv(key_cache.data_ptr(), value_cache.data_ptr(), weight_cache.data_ptr<float>(),
                                   block_tables.data_ptr<int>(), context_lens.data_ptr<int>(), kept_positions.data_ptr<int>(),

@@ -14,17 +14,19 @@
 // bits, made to order like whole numbers, are searched for the last one that
 // stays in three passes of 11, 11 and 10 bits (a histogram in LDS each), then
 // every wave counts its stretch, and lists it behind the others'.  Up to kKeys
-// weights are held in LDS; longer contexts read them from L2 again.
+// weights are held in LDS with their part of the block table, and moved from
+// there; longer contexts read the rest from L2 in every pass.
 //
-// pa_evict_move_kernel: one wave to 1 KiB of every block of a (sequence, kv head):
-// a run of keys' chunks, of values' rows, or the weights.  It walks the blocks
-// from the first that loses a position: a slot is written from a position at or
-// behind it, so whatever is still to be read is never overwritten, and waves
-// never share a byte.  Keys go straight to their slots, 16 bytes each; values,
-// whose positions lie side by side in a row, are collected in LDS until a block
-// is full.  Bound by HBM: with a quarter of the positions kept at random every
-// 128-byte line of the old blocks holds one that stays, so the whole of them is
-// read (the values' rows of a block even with one position in sixteen).
+// pa_evict_move_kernel: one wave to 64 pieces of 16 bytes of every 16 slots of a
+// (sequence, kv head): 4 chunks of the keys, or as many rows of the values.  It walks
+// the slots from the first that changes, and takes each from where the list says: a
+// slot comes from a position at or behind it, so what later slots need is never
+// overwritten, and waves never share a byte.  A key's piece is one load and one store;
+// a value's is put together of single elements, as positions lie side by side in a row.
+// Several steps' loads are on their way at once, the list and the block table one and
+// two steps ahead.  Bound by HBM: with a quarter of the positions kept at random every
+// 128-byte line of the old blocks holds one that stays, so the whole of them is read
+// (the values' rows of a block even with one position in sixteen).
 #include "pa_common.h"
 
 namespace pa {
@@ -36,21 +38,21 @@ struct EvictArgs {
   const int32_t* tables;
   const int32_t* ctx;
   int32_t* kept;            // [num_seqs, heads, budget]
-  uint64_t* masks;          // [num_seqs, heads, words]: which of 64 positions stay
-  int32_t* ranks;           // [num_seqs, heads, words]: how many stay before them
-  int32_t* first;           // [num_seqs, heads]: the first block that loses a position, -1: none
-  int heads, block_bits, num_blocks, table_width, max_ctx, budget, recent, words;
+  int32_t* first;           // [num_seqs, heads]: the first position that goes, -1: none
+  int heads, head_size, block_bits, num_blocks, table_width, max_ctx, budget, recent;
   int tile_bytes;           // of one head's share of a block: head_size * block * element size
-  int slices;               // ceil(tile_bytes / 1024)
-  int64_t tasks;            // (sequence, head, slice) of the move
+  int key_tasks, value_tasks;  // waves of a (sequence, head): for its keys, for its values, and one for its weights
+  int64_t tasks;
 };
 
 namespace {
 
 constexpr int kThreads = 1024;
 constexpr int kWaves = kThreads / 64;
-constexpr int kKeys = 8192;
+constexpr int kKeys = 16384;
+constexpr int kEntries = kKeys / 8;  // of the block table, at the smallest block
 constexpr int kBins = 2048;
+constexpr int kBatch = 8;            // loads of a thread on their way at once
 
 // A weight as a whole number of the same order: NaN first of all, then by value, both zeros alike.
 __device__ __forceinline__ uint32_t order_key(uint32_t bits) {
@@ -76,20 +78,50 @@ __global__ void __launch_bounds__(kThreads) pa_evict_select_kernel(const EvictAr
     if (tid == 0) a.first[sh] = -1;
     return;
   }
-  __shared__ uint32_t sm_key[kKeys];
+  __shared__ uint32_t sm_bits[kKeys];
+  __shared__ int32_t sm_table[kEntries];
   __shared__ uint32_t sm_hist[kBins];
   __shared__ uint32_t sm_scan[kWaves];
   __shared__ uint32_t sm_bin, sm_need;
   __shared__ int sm_gt[kWaves], sm_eq[kWaves], sm_first;
-  const int candidates = n - a.recent;
-  const uint32_t* weights = reinterpret_cast<const uint32_t*>(a.weights);
-  const auto fetch = [&](int p) {
-    const int64_t b = table[p >> a.block_bits];
-    return order_key(weights[((b * a.heads + head) << a.block_bits) + (p & ((1 << a.block_bits) - 1))]);
-  };
-  for (int p = tid; p < candidates && p < kKeys; p += kThreads) sm_key[p] = fetch(p);
+  const int candidates = n - a.recent, held = n < kKeys ? n : kKeys;
+  uint32_t* weights = reinterpret_cast<uint32_t*>(a.weights);
+  const int within = (1 << a.block_bits) - 1;
+  for (int e = tid; e <= (held - 1) >> a.block_bits; e += kThreads) sm_table[e] = table[e];
   if (tid == 0) sm_first = n;
-  const auto key = [&](int p) { return p < kKeys ? sm_key[p] : fetch(p); };
+  __syncthreads();
+  const auto slot = [&](int block, int p) { return (((int64_t)block * a.heads + head) << a.block_bits) + (p & within); };
+  for (int p0 = tid; p0 < held; p0 += kBatch * kThreads) {
+    uint32_t v[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; i++) {
+      const int p = p0 + i * kThreads < held ? p0 + i * kThreads : held - 1;
+      v[i] = weights[slot(sm_table[p >> a.block_bits], p)];
+    }
+#pragma unroll
+    for (int i = 0; i < kBatch; i++)
+      if (p0 + i * kThreads < held) sm_bits[p0 + i * kThreads] = v[i];
+  }
+  __syncthreads();
+  // positions tid, tid + kThreads, ... from LDS, then from memory, several at once
+  const auto each_key = [&](auto use) {
+    for (int p = tid; p < candidates && p < kKeys; p += kThreads) use(order_key(sm_bits[p]));
+    for (int p0 = kKeys + tid; p0 < candidates; p0 += kBatch * kThreads) {
+      int32_t b[kBatch];
+      uint32_t v[kBatch];
+#pragma unroll
+      for (int i = 0; i < kBatch; i++) b[i] = table[(p0 + i * kThreads < candidates ? p0 + i * kThreads : candidates - 1) >> a.block_bits];
+#pragma unroll
+      for (int i = 0; i < kBatch; i++) {
+        const int p = p0 + i * kThreads < candidates ? p0 + i * kThreads : candidates - 1;
+        v[i] = weights[slot(b[i], p)];
+      }
+#pragma unroll
+      for (int i = 0; i < kBatch; i++)
+        if (p0 + i * kThreads < candidates) use(order_key(v[i]));
+    }
+  };
+  const auto key = [&](int p) { return order_key(p < kKeys ? sm_bits[p] : weights[slot(table[p >> a.block_bits], p)]); };
 
   uint32_t limit = 0, need = (uint32_t)(a.budget - a.recent);  // need: how many of the keys with limit's upper bits stay
   const bool any = need > 0;
@@ -99,10 +131,9 @@ __global__ void __launch_bounds__(kThreads) pa_evict_select_kernel(const EvictAr
       const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0), bits = pass == 2 ? 10 : 11;
       for (int i = tid; i < kBins; i += kThreads) sm_hist[i] = 0;
       __syncthreads();
-      for (int p = tid; p < candidates; p += kThreads) {
-        const uint32_t k = key(p);
+      each_key([&](uint32_t k) {
         if (pass == 0 || (k >> (shift + bits)) == (limit >> (shift + bits))) atomicAdd(&sm_hist[(k >> shift) & ((1u << bits) - 1u)], 1u);
-      }
+      });
       __syncthreads();
       // bins from the highest down, two to a thread: the one in which the need-th key lies
       const uint32_t hi = sm_hist[kBins - 1 - 2 * tid], lo = sm_hist[kBins - 2 - 2 * tid];
@@ -115,7 +146,8 @@ __global__ void __launch_bounds__(kThreads) pa_evict_select_kernel(const EvictAr
       if (lane == 63) sm_scan[wave] = sum;
       __syncthreads();
       uint32_t before = 0;
-      for (int w = 0; w < wave; w++) before += sm_scan[w];
+#pragma unroll
+      for (int w = 0; w < kWaves; w++) before += w < wave ? sm_scan[w] : 0u;  // all reads at once
       before += sum - (hi + lo);
       if (before < need && need <= before + hi + lo) {
         const bool in_hi = need <= before + hi;
@@ -157,9 +189,10 @@ __global__ void __launch_bounds__(kThreads) pa_evict_select_kernel(const EvictAr
   }
   __syncthreads();
   int run = 0, ties = 0;
-  for (int w = 0; w < wave; w++) {
-    run += sm_gt[w];
-    ties += sm_eq[w];
+#pragma unroll
+  for (int w = 0; w < kWaves; w++) {
+    run += w < wave ? sm_gt[w] : 0;
+    ties += w < wave ? sm_eq[w] : 0;
   }
   const int wanted = any ? (int)need : 0;
   run += ties < wanted ? ties : wanted;
@@ -172,10 +205,10 @@ __global__ void __launch_bounds__(kThreads) pa_evict_select_kernel(const EvictAr
     const bool stays = gt || (eq && ties + __popcll(em & below) < wanted);
     ties += __popcll(em);
     const uint64_t mask = __ballot(stays);
-    if (stays) kept[run + __popcll(mask & below)] = p + lane;
-    if (lane == 0) {
-      a.masks[(int64_t)sh * a.words + (p >> 6)] = mask;
-      a.ranks[(int64_t)sh * a.words + (p >> 6)] = run;
+    if (stays) {
+      const int to = run + __popcll(mask & below);
+      kept[to] = p + lane;
+      if (n <= kKeys) weights[slot(sm_table[to >> a.block_bits], to)] = sm_bits[p + lane];
     }
     run += __popcll(mask);
     if (dropped == n && ~mask != 0) {
@@ -185,144 +218,171 @@ __global__ void __launch_bounds__(kThreads) pa_evict_select_kernel(const EvictAr
   }
   if (lane == 0 && dropped < n) atomicMin(&sm_first, dropped);
   __syncthreads();
-  if (tid == 0) a.first[sh] = sm_first >> a.block_bits;
+  if (tid == 0) a.first[sh] = sm_first;
 }
 
-constexpr int kAhead = 4;  // blocks whose loads are in flight beside the ones being placed
+constexpr int kSlots = 16;  // a wave's step
 
-// X: elements of 16 bytes.  The tables that no store of the kernel touches are arguments of their
-// own: their loads, the same for all lanes, then go through the scalar cache and its counter, and no
-// wait for them waits for the blocks that are on their way.
+// X: elements of 16 bytes.  U: steps whose loads are on their way at once.
 template <typename T, int X>
 __global__ void __launch_bounds__(256)
-pa_evict_move_kernel(const EvictArgs a, const int32_t* __restrict__ tables, const int32_t* __restrict__ ctx,
-                     const uint64_t* __restrict__ all_masks, const int32_t* __restrict__ all_ranks,
+pa_evict_move_kernel(const EvictArgs a, const int32_t* __restrict__ tables, const int32_t* __restrict__ all_kept,
                      const int32_t* __restrict__ firsts, char* __restrict__ kc, char* __restrict__ vc,
                      float* __restrict__ weights) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t task = (int64_t)blockIdx.x * 4 + wave;
   if (task >= a.tasks) return;
-  const int kinds = 2 * a.slices + 1;
+  const int kinds = a.key_tasks + a.value_tasks + 1;
   const int sh = (int)(task / kinds), kind = (int)(task - (int64_t)sh * kinds);
   const int first = firsts[sh];
   if (first < 0) return;
   const int seq = sh / a.heads, head = sh - seq * a.heads;
-  const int n = ctx[seq], B = 1 << a.block_bits, blocks = (n + B - 1) >> a.block_bits;
+  const int bits = a.block_bits, B = 1 << bits, last = a.budget - 1;
   const int32_t* table = tables + (int64_t)seq * a.table_width;
-  const uint64_t* masks = all_masks + (int64_t)sh * a.words;
-  const int32_t* ranks = all_ranks + (int64_t)sh * a.words;
+  const int32_t* kept = all_kept + (int64_t)sh * a.budget;
+  const auto within = [&](int slot) { return slot < last ? slot : last; };  // slots past the last: the last again
 
-  if (kind == 2 * a.slices) {  // weights, 64 positions at a time
-    const auto slot = [&](int p) { return ((((int64_t)table[p >> a.block_bits]) * a.heads + head) << a.block_bits) + (p & (B - 1)); };
-    const int last = (n - 1) >> 6;
-    int w = (first << a.block_bits) >> 6;
-    float next = 0.f;
-    if (w * 64 + lane < n) next = weights[slot(w * 64 + lane)];
-    for (; w <= last; w++) {
-      const float v = next;
-      if ((w + 1) * 64 + lane < n) next = weights[slot((w + 1) * 64 + lane)];
-      const uint64_t mask = masks[w];
-      if ((mask >> lane) & 1) weights[slot(ranks[w] + __popcll(mask & ((1ull << lane) - 1ull)))] = v;
+  if (kind == a.key_tasks + a.value_tasks) {  // the weights of a context that was too long for the selection's LDS
+    if (a.ctx[seq] <= kKeys) return;
+    const auto at = [&](int block, int p) { return (((int64_t)block * a.heads + head) << bits) + (p & (B - 1)); };
+    constexpr int U = 8;
+    for (int w0 = first & ~63; w0 <= last; w0 += 64 * U) {
+      int p[U];
+      float v[U];
+      int64_t to[U];
+#pragma unroll
+      for (int u = 0; u < U; u++) p[u] = kept[within(w0 + 64 * u + lane)];
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        const int slot = within(w0 + 64 * u + lane);
+        v[u] = weights[at(table[p[u] >> bits], p[u])];
+        to[u] = at(table[slot >> bits], slot);
+      }
+#pragma unroll
+      for (int u = 0; u < U; u++)
+        if (w0 + 64 * u + lane <= last) weights[to[u]] = v[u];
     }
     return;
   }
-  const bool values = kind >= a.slices;
-  const int at = (values ? kind - a.slices : kind) * 1024 + lane * 16;  // this lane's bytes of the tile
-  const bool mine = at < a.tile_bytes;
-  char* base = (values ? vc : kc) + (int64_t)head * a.tile_bytes;
   const int64_t block_bytes = (int64_t)a.heads * a.tile_bytes;
-  const int vec = at >> 4;
-  const int per_row = B / X;                                            // values: vectors of a row
-  const int token = values ? (vec & (per_row - 1)) * X : vec & (B - 1);  // the (first) token of this lane's vector
-  __shared__ __attribute__((aligned(16))) T sm[4][128 * X];
-  T* strip = sm[wave] + (lane / per_row) * 2 * B;                       // this lane's row: two blocks of tokens
+  // 64 slots at a time, one to a lane: where it is (block * B + offset) and where it comes from, in pages of
+  // which the next is on its way and the list for the one behind it too.  Lanes get them from each other: as
+  // loads of their own they would be two to an element, and the address units' time is what values are bound by.
+  struct Page { int position, from, to; };
+  const auto ask = [&](int w) { return kept[within(w + lane)]; };
+  const auto look_up = [&](int position, int w) {
+    Page r;
+    r.position = position;
+    r.from = table[position >> bits];
+    r.to = table[within(w + lane) >> bits];
+    return r;
+  };
+  const auto source = [&](const Page& g) { return g.from << bits | (g.position & (B - 1)); };
+  const auto target = [&](const Page& g, int w) { return g.to << bits | (within(w + lane) & (B - 1)); };
+  const auto lane_of = [](int v, int l) { return __builtin_amdgcn_ds_bpermute(l * 4, v); };
+  const int w0 = first & ~(kSlots - 1);
 
-  const auto bits_of = [&](int b, int* rank) {  // which tokens of block b stay, and the slot of the first
-    const int p = b << a.block_bits;
-    const uint64_t mask = masks[p >> 6];
-    *rank = ranks[p >> 6] + __popcll(mask & ((1ull << (p & 63)) - 1ull));
-    return (uint32_t)(mask >> (p & 63)) & (B == 32 ? 0xffffffffu : (1u << B) - 1u);
-  };
-  const auto fetch = [&](int b) {
-    u32x4 v = {0, 0, 0, 0};
-    if (b < blocks) {
-      int rank;
-      if (bits_of(b, &rank) != 0 && mine) v = *reinterpret_cast<const u32x4*>(base + (int64_t)table[b] * block_bytes + at);
+  if (kind < a.key_tasks) {
+    constexpr int G = 2, U = 64 / kSlots;  // pages, and steps of a page
+    const int t = lane & (kSlots - 1), chunk = kind * 4 + lane / kSlots;
+    const bool mine = chunk < a.head_size / X;
+    char* base = kc + (int64_t)head * a.tile_bytes + (mine ? chunk : 0) * B * 16;
+    const auto address = [&](int slot) { return base + (int64_t)(slot >> bits) * block_bytes + (slot & (B - 1)) * 16; };
+    Page page[G];
+    int next[G];
+#pragma unroll
+    for (int q = 0; q < G; q++) {
+      page[q] = look_up(ask(w0 + 64 * q), w0 + 64 * q);
+      next[q] = ask(w0 + 64 * (G + q));
     }
-    return v;
-  };
-  const auto flush = [&](int slot_block) {
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    const u32x4 v = *reinterpret_cast<const u32x4*>(strip + (slot_block & 1) * B + token);
-    if (mine) *reinterpret_cast<u32x4*>(base + (int64_t)table[slot_block] * block_bytes + at) = v;
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  };
-  u32x4 ahead[kAhead];
+    for (int w = w0; w <= last; w += 64 * G) {
+      u32x4 v[G][U];
+      char* dst[G][U];
 #pragma unroll
-  for (int u = 0; u < kAhead; u++) ahead[u] = fetch(first + u);
-  int filled = first << a.block_bits;  // slots done
-  for (int b0 = first; b0 < blocks; b0 += kAhead) {
-    u32x4 now[kAhead];
+      for (int q = 0; q < G; q++) {
+        const int from = source(page[q]), to = target(page[q], w + 64 * q);
 #pragma unroll
-    for (int u = 0; u < kAhead; u++) now[u] = ahead[u];
-#pragma unroll
-    for (int u = 0; u < kAhead; u++) ahead[u] = fetch(b0 + kAhead + u);
-#pragma unroll
-    for (int u = 0; u < kAhead; u++) {
-      if (b0 + u >= blocks) break;
-      int rank;
-      const uint32_t bits = bits_of(b0 + u, &rank);
-      if (bits == 0) continue;
-      const int e0 = rank >> a.block_bits;
-      if (!values) {
-        const int e1 = e0 + 1 < blocks ? e0 + 1 : e0;
-        const int to = rank + __popc(bits & ((1u << token) - 1u));
-        const int64_t t0 = table[e0], t1 = table[e1];
-        if (mine && ((bits >> token) & 1u))
-          *reinterpret_cast<u32x4*>(base + ((to >> a.block_bits) == e0 ? t0 : t1) * block_bytes + at + ((to & (B - 1)) - token) * 16) = now[u];
-      } else {
-#pragma unroll
-        for (int i = 0; i < X; i++) {
-          const T e = (T)(X == 4 ? now[u][i & 3] : now[u][i >> 1] >> (16 * (i & 1)));
-          if ((bits >> (token + i)) & 1u) strip[(rank + __popc(bits & ((1u << (token + i)) - 1u))) & (2 * B - 1)] = e;
+        for (int u = 0; u < U; u++) {
+          v[q][u] = *reinterpret_cast<const u32x4*>(address(lane_of(from, u * kSlots + t)));
+          dst[q][u] = address(lane_of(to, u * kSlots + t));
         }
-        filled = rank + __popc(bits);
-        if ((rank ^ filled) >> a.block_bits) flush(e0);
+      }
+      Page ahead[G];
+#pragma unroll
+      for (int q = 0; q < G; q++) ahead[q] = look_up(next[q], w + 64 * (G + q));
+#pragma unroll
+      for (int q = 0; q < G; q++) next[q] = ask(w + 64 * (2 * G + q));
+#pragma unroll
+      for (int q = 0; q < G; q++)
+#pragma unroll
+        for (int u = 0; u < U; u++)
+          if (mine && w + 64 * q + kSlots * u + t <= last) *reinterpret_cast<u32x4*>(dst[q][u]) = v[q][u];
+#pragma unroll
+      for (int q = 0; q < G; q++) page[q] = ahead[q];
+    }
+    return;
+  }
+
+  constexpr int VECS = kSlots / X, U = 64 / kSlots;
+  const int first_slot = (lane & (VECS - 1)) * X, row = (kind - a.key_tasks) * (64 / VECS) + lane / VECS;
+  const bool mine = row < a.head_size;
+  char* base = vc + (int64_t)head * a.tile_bytes + (int64_t)(mine ? row : 0) * B * (int)sizeof(T);
+  const auto address = [&](int slot) { return base + (int64_t)(slot >> bits) * block_bytes + (slot & (B - 1)) * (int)sizeof(T); };
+  constexpr int G = 2;
+  Page page[G];
+  int next[G];
+#pragma unroll
+  for (int q = 0; q < G; q++) {
+    page[q] = look_up(ask(w0 + 64 * q), w0 + 64 * q);
+    next[q] = ask(w0 + 64 * (G + q));
+  }
+  for (int w = w0; w <= last; w += 64 * G) {
+    T v[G][U][X];
+    char* dst[G][U];
+#pragma unroll
+    for (int q = 0; q < G; q++) {
+      const int from = source(page[q]), to = target(page[q], w + 64 * q);
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+#pragma unroll
+        for (int i = 0; i < X; i++) v[q][u][i] = *reinterpret_cast<const T*>(address(lane_of(from, u * kSlots + first_slot + i)));
+        dst[q][u] = address(lane_of(to, u * kSlots + first_slot));
       }
     }
-  }
-  if (values && (filled & (B - 1))) {  // the last block's slots behind the budget stay as they are
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    const int slot_block = filled >> a.block_bits, left = (filled & (B - 1)) - token;
-    T* to = reinterpret_cast<T*>(base + (int64_t)table[slot_block] * block_bytes + at);
+    Page ahead[G];
 #pragma unroll
-    for (int i = 0; i < X; i++)
-      if (mine && i < left) to[i] = strip[(slot_block & 1) * B + token + i];
+    for (int q = 0; q < G; q++) ahead[q] = look_up(next[q], w + 64 * (G + q));
+#pragma unroll
+    for (int q = 0; q < G; q++) next[q] = ask(w + 64 * (2 * G + q));
+#pragma unroll
+    for (int q = 0; q < G; q++)
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        const int left = last + 1 - (w + 64 * q + kSlots * u + first_slot);  // slots of this lane within the budget
+        if (mine && left >= X) {
+          u32x4 r;
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+            r[i] = X == 4 ? (uint32_t)v[q][u][i] : (uint32_t)v[q][u][(2 * i) % X] | (uint32_t)v[q][u][(2 * i + 1) % X] << 16;
+          *reinterpret_cast<u32x4*>(dst[q][u]) = r;
+        } else if (mine && left > 0) {  // the slots behind the budget stay as they are
+#pragma unroll
+          for (int i = 0; i < X; i++)
+            if (i < left) reinterpret_cast<T*>(dst[q][u])[i] = v[q][u][i];
+        }
+      }
+#pragma unroll
+    for (int q = 0; q < G; q++) page[q] = ahead[q];
   }
 }
 
-struct EvictPlan {
-  int words;
-  size_t mask_bytes, rank_bytes, first_bytes;
-  size_t bytes() const { return mask_bytes + rank_bytes + first_bytes; }
-};
-
-EvictPlan evict_plan(int num_seqs, int heads, int max_ctx) {
-  EvictPlan p;
-  p.words = (max_ctx + 63) / 64;
-  const size_t cells = (size_t)num_seqs * heads;
-  p.mask_bytes = cells * p.words * 8;
-  p.rank_bytes = (cells * p.words * 4 + 15) / 16 * 16;
-  p.first_bytes = (cells * 4 + 15) / 16 * 16;
-  return p;
-}
+size_t evict_bytes(int num_seqs, int heads) { return ((size_t)num_seqs * heads * 4 + 15) / 16 * 16; }
 
 }  // namespace
 }  // namespace pa
 
-extern "C" size_t pa_evict_workspace_bytes(int num_seqs, int num_kv_heads, int max_context_len) {
-  if (num_seqs <= 0 || num_kv_heads <= 0 || max_context_len < 0) return 0;
-  return pa::evict_plan(num_seqs, num_kv_heads, max_context_len).bytes();
+extern "C" size_t pa_evict_workspace_bytes(int num_seqs, int num_kv_heads) {
+  return num_seqs <= 0 || num_kv_heads <= 0 ? 0 : pa::evict_bytes(num_seqs, num_kv_heads);
 }
 
 extern "C" int pa_evict_cached_kv(void* key_cache, void* value_cache, float* weight_cache, const int32_t* block_tables,
@@ -352,9 +412,9 @@ extern "C" int pa_evict_cached_kv(void* key_cache, void* value_cache, float* wei
   PA_REQUIRE((int64_t)max_num_blocks_per_seq * block_size >= max_context_len,
              "%s: block tables of %d blocks cannot hold max_context_len %d", what, max_num_blocks_per_seq, max_context_len);
   PA_REQUIRE(max_context_len <= (1 << 30), "%s: max_context_len %d is too large", what, max_context_len);
-  const EvictPlan p = evict_plan(num_seqs, num_kv_heads, max_context_len);
-  PA_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= p.bytes(),
-             "%s: workspace of %zu bytes, 16-byte aligned, needed", what, p.bytes());
+  PA_REQUIRE((int64_t)num_blocks * block_size <= 0x7fffffff, "%s: more than 2^31 slots", what);
+  PA_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= evict_bytes(num_seqs, num_kv_heads),
+             "%s: workspace of %zu bytes, 16-byte aligned, needed", what, evict_bytes(num_seqs, num_kv_heads));
   const int64_t cells = (int64_t)num_seqs * num_kv_heads;
   EvictArgs a = {};
   a.kc = static_cast<char*>(key_cache);
@@ -363,10 +423,7 @@ extern "C" int pa_evict_cached_kv(void* key_cache, void* value_cache, float* wei
   a.tables = block_tables;
   a.ctx = context_lens;
   a.kept = kept_positions;
-  char* ws = static_cast<char*>(workspace);
-  a.masks = reinterpret_cast<uint64_t*>(ws);
-  a.ranks = reinterpret_cast<int32_t*>(ws + p.mask_bytes);
-  a.first = reinterpret_cast<int32_t*>(ws + p.mask_bytes + p.rank_bytes);
+  a.first = static_cast<int32_t*>(workspace);
   a.heads = num_kv_heads;
   a.block_bits = block_size == 8 ? 3 : (block_size == 16 ? 4 : 5);
   a.num_blocks = num_blocks;
@@ -374,10 +431,11 @@ extern "C" int pa_evict_cached_kv(void* key_cache, void* value_cache, float* wei
   a.max_ctx = max_context_len;
   a.budget = budget;
   a.recent = num_recent;
-  a.words = p.words;
+  a.head_size = head_size;
   a.tile_bytes = head_size * block_size * elem_size(dtype);
-  a.slices = (a.tile_bytes + 1023) / 1024;
-  a.tasks = cells * (2 * a.slices + 1);
+  a.key_tasks = (head_size / x + 3) / 4;
+  a.value_tasks = (head_size + 4 * x - 1) / (4 * x);  // 64 / (16 / x) rows each
+  a.tasks = cells * (a.key_tasks + a.value_tasks + 1);
   PA_REQUIRE(cells <= 0x7fffffff && (a.tasks + 3) / 4 <= 0x7fffffff, "%s: too many heads for one launch", what);
   hipStream_t st = static_cast<hipStream_t>(stream);
   hipLaunchKernelGGL(pa_evict_select_kernel, dim3((unsigned)cells), dim3(kThreads), 0, st, a);
@@ -385,9 +443,9 @@ extern "C" int pa_evict_cached_kv(void* key_cache, void* value_cache, float* wei
   if (max_context_len <= budget) return PA_OK;  // no sequence can lose a position
   const dim3 grid((unsigned)((a.tasks + 3) / 4));
   if (elem_size(dtype) == 4)
-    hipLaunchKernelGGL((pa_evict_move_kernel<uint32_t, 4>), grid, dim3(256), 0, st, a, a.tables, a.ctx, a.masks, a.ranks, a.first, a.kc, a.vc, a.weights);
+    hipLaunchKernelGGL((pa_evict_move_kernel<uint32_t, 4>), grid, dim3(256), 0, st, a, a.tables, a.kept, a.first, a.kc, a.vc, a.weights);
   else
-    hipLaunchKernelGGL((pa_evict_move_kernel<uint16_t, 8>), grid, dim3(256), 0, st, a, a.tables, a.ctx, a.masks, a.ranks, a.first, a.kc, a.vc, a.weights);
+    hipLaunchKernelGGL((pa_evict_move_kernel<uint16_t, 8>), grid, dim3(256), 0, st, a, a.tables, a.kept, a.first, a.kc, a.vc, a.weights);
   PA_CHECK_LAUNCH(what);
   return PA_OK;
 }
