@@ -13,13 +13,16 @@
 // type): a 16-bit table would put an error of 2^-9 on every angle's cosine,
 // which is as much as the result's own rounding.
 //
-// One pass over the rows, bound by HBM for prompts and by the launch for the
-// steps of a small batch.  2^k lanes own a head (k such that a lane holds one
-// vector pair, and one vector of the part that is not rotated): a head's sum of
-// squares is then k exchanges between neighbouring lanes, and both elements of a
-// pair are in one lane in both layouts.  A lane keeps its table entries for all
-// the heads of a token that it visits: the row is fetched once per wave, not
-// once per head.
+// One pass over the rows, bound by HBM for prompts (8192 tokens of 40 + 40 heads
+// of 128 with norms, fp16: 70 us = 4.9 TB/s of the 5.9 that an in-place pass over
+// plain memory reaches) and by the launch for the steps of a small batch (8 tokens
+// 2.7 us, 256 tokens with norms 3.7).  2^k lanes own a head (k such that a lane holds
+// two vectors of the rotated part, and one of the rest): a head's sum of squares is
+// then k exchanges between lanes, and both elements of a pair are in one lane in both
+// layouts.  A lane keeps its table entries for all the heads of a token that it
+// visits: the row is fetched once per wave, not once per head.  Two heads in a lane's
+// hand at once were slower (84 us), streaming loads and stores too where a part of
+// every head is rotated (43 us against 37).
 #include "pa_common.h"
 #include "pa_exact_math.h"
 
@@ -66,93 +69,119 @@ __device__ __forceinline__ void store_rounded(T* p, const float* f) {
   *reinterpret_cast<Vec<T, N>*>(p) = x;
 }
 
-// W: elements of a vector.  In the half layout a lane's pairs are the vectors at
-// W * i and rot_dim / 2 + W * i, in the interleaved one the vectors at 2 W i and
-// 2 W i + W, so a lane holds W pairs either way.  grid = (tokens, slices of the heads).
+// the W / 2 pairs of one vector
+template <int W>
+__device__ __forceinline__ void turn_inside(float* v, const float* c, const float* s) {
+#pragma unroll
+  for (int e = 0; e < W / 2; e++) {
+    const float p = v[2 * e], q = v[2 * e + 1];
+    v[2 * e] = __builtin_fmaf(p, c[e], -(q * s[e]));
+    v[2 * e + 1] = __builtin_fmaf(q, c[e], p * s[e]);
+  }
+}
+
+// W: elements of a vector.  A lane's two vectors are W * i and rot_dim / 2 + W * i in both layouts, so that
+// neighbouring lanes read neighbouring memory: W pairs across them in the half layout, W / 2 pairs within each in
+// the interleaved one (W = 1: the two elements of one pair).  The chain of loads is kept short: a token's first
+// heads are on their way before its position is known, its next ones while the last are worked on, and the
+// weights while a sum is exchanged.  grid = (tokens, slices of the heads).
 template <typename T, typename TT, int W, bool INTERLEAVED, bool NORM>
 __global__ void __launch_bounds__(256)
 pa_rotary_kernel(const RotaryArgs a) {
   const int token = blockIdx.x;
-  const int64_t pos = a.positions[token];
-  if (pos < 0) return;  // a padded row
+  constexpr bool INSIDE = INTERLEAVED && W > 1;  // pairs within a vector
   const int half = a.rot_dim >> 1;
   const int lane = threadIdx.x & ((1 << a.lane_bits) - 1);
   const int slot = (int)((blockIdx.y * blockDim.x + threadIdx.x) >> a.lane_bits);
   const int slots = (int)((gridDim.y * blockDim.x) >> a.lane_bits);
   const int heads = a.num_heads[0] + a.num_heads[1];
+  if (slot >= heads) return;
   const bool has_pair = W * lane < half;
-  const int ia = INTERLEAVED ? 2 * W * lane : W * lane;
-  const int ib = INTERLEAVED ? ia + W : half + ia;
+  const int ia = INTERLEAVED && !INSIDE ? 2 * lane : W * lane;
+  const int ib = INTERLEAVED && !INSIDE ? ia + 1 : half + ia;
   const int it = a.rot_dim + W * lane;
   const bool has_tail = NORM && it < a.head_size;
+  typedef Vec<T, W> V;
 
+  struct Head { T* base; const T* weight; V x, y, t; };
+  const auto fetch = [&](int h) {
+    Head r;
+    const int w = h >= a.num_heads[0];
+    r.base = static_cast<T*>(a.rows[w]) + (int64_t)token * a.stride[w] + (int64_t)(h - (w ? a.num_heads[0] : 0)) * a.head_size;
+    r.weight = static_cast<const T*>(a.weight[w]);
+    // lanes without a part of the head read its first elements
+    r.x = *reinterpret_cast<const V*>(r.base + (has_pair ? ia : 0));
+    r.y = *reinterpret_cast<const V*>(r.base + (has_pair ? ib : 0));
+    if (NORM) r.t = *reinterpret_cast<const V*>(r.base + (has_tail ? it : 0));
+    return r;
+  };
+  Head next = fetch(slot);
+  const int64_t pos = a.positions[token];
+  if (pos < 0) return;  // a padded row
+
+  // INSIDE: the first vector's W / 2 pairs, then the second's
   float c[W], s[W];
 #pragma unroll
   for (int e = 0; e < W; e++) c[e] = s[e] = 0.f;
   if (has_pair) {
     if (pos < a.max_position) {
-      const TT* row = static_cast<const TT*>(a.table) + pos * a.rot_dim + W * lane;
-      load_table<TT, W>(row, c);
-      load_table<TT, W>(row + half, s);
+      const TT* row = static_cast<const TT*>(a.table) + pos * a.rot_dim;
+      if constexpr (INSIDE) {
+        load_table<TT, W / 2>(row + ia / 2, c);
+        load_table<TT, W / 2>(row + ib / 2, c + W / 2);
+        load_table<TT, W / 2>(row + half + ia / 2, s);
+        load_table<TT, W / 2>(row + half + ib / 2, s + W / 2);
+      } else {
+        load_table<TT, W>(row + W * lane, c);
+        load_table<TT, W>(row + half + W * lane, s);
+      }
     } else {  // no such row: the caller's mistake must not pass for a result
 #pragma unroll
       for (int e = 0; e < W; e++) c[e] = s[e] = __builtin_nanf("");
     }
   }
   for (int h = slot; h < heads; h += slots) {
-    const int w = h >= a.num_heads[0];
-    T* base = static_cast<T*>(a.rows[w]) + (int64_t)token * a.stride[w] +
-              (int64_t)(h - (w ? a.num_heads[0] : 0)) * a.head_size;
+    const Head now = next;
+    next = fetch(h + slots < heads ? h + slots : h);  // behind the last, the last again
     float x[W], y[W], t[W];
 #pragma unroll
-    for (int e = 0; e < W; e++) x[e] = y[e] = t[e] = 0.f;
-    if (has_pair) {
-      load_f32<T, W>(base + ia, x);
-      load_f32<T, W>(base + ib, y);
+    for (int e = 0; e < W; e++) {
+      x[e] = has_pair ? Num<T>::to(now.x.v[e]) : 0.f;
+      y[e] = has_pair ? Num<T>::to(now.y.v[e]) : 0.f;
+      if (NORM) t[e] = has_tail ? Num<T>::to(now.t.v[e]) : 0.f;
     }
-    if (has_tail) load_f32<T, W>(base + it, t);
     if (NORM) {
+      float gx[W], gy[W], gt[W];
+      load_f32<T, W>(now.weight + (has_pair ? ia : 0), gx);
+      load_f32<T, W>(now.weight + (has_pair ? ib : 0), gy);
+      load_f32<T, W>(now.weight + (has_tail ? it : 0), gt);
       float ss = 0.f;
 #pragma unroll
       for (int e = 0; e < W; e++) ss = __builtin_fmaf(x[e], x[e], __builtin_fmaf(y[e], y[e], __builtin_fmaf(t[e], t[e], ss)));
       for (int off = (1 << a.lane_bits) >> 1; off >= 1; off >>= 1) ss += __shfl_xor(ss, off);
       const float r = 1.0f / sqrtf(ss / (float)a.head_size + a.epsilon);
-      const T* weight = static_cast<const T*>(a.weight[w]);
-      float g[W];
-      if (has_pair) {
-        load_f32<T, W>(weight + ia, g);
 #pragma unroll
-        for (int e = 0; e < W; e++) x[e] *= r * g[e];
-        load_f32<T, W>(weight + ib, g);
-#pragma unroll
-        for (int e = 0; e < W; e++) y[e] *= r * g[e];
+      for (int e = 0; e < W; e++) {
+        x[e] *= r * gx[e];
+        y[e] *= r * gy[e];
+        t[e] *= r * gt[e];
       }
-      if (has_tail) {
-        load_f32<T, W>(weight + it, g);
-#pragma unroll
-        for (int e = 0; e < W; e++) t[e] *= r * g[e];
-        store_rounded<T, W>(base + it, t);
-      }
+      if (has_tail) store_rounded<T, W>(now.base + it, t);
     }
     if (has_pair) {
-      float u[2 * W];
-      if (INTERLEAVED) {  // x then y hold 2 W elements in order: pair e is (2 e, 2 e + 1)
-#pragma unroll
-        for (int e = 0; e < W; e++) {
-          const float p = 2 * e < W ? x[(2 * e) % W] : y[(2 * e) % W];
-          const float q = W == 1 ? y[0] : (2 * e < W ? x[(2 * e + 1) % W] : y[(2 * e + 1) % W]);
-          u[2 * e] = __builtin_fmaf(p, c[e], -(q * s[e]));
-          u[2 * e + 1] = __builtin_fmaf(q, c[e], p * s[e]);
-        }
+      if constexpr (INSIDE) {
+        turn_inside<W>(x, c, s);
+        turn_inside<W>(y, c + W / 2, s + W / 2);
       } else {
 #pragma unroll
         for (int e = 0; e < W; e++) {
-          u[e] = __builtin_fmaf(x[e], c[e], -(y[e] * s[e]));
-          u[W + e] = __builtin_fmaf(y[e], c[e], x[e] * s[e]);
+          const float p = x[e], q = y[e];
+          x[e] = __builtin_fmaf(p, c[e], -(q * s[e]));
+          y[e] = __builtin_fmaf(q, c[e], p * s[e]);
         }
       }
-      store_rounded<T, W>(base + ia, u);
-      store_rounded<T, W>(base + ib, u + W);
+      store_rounded<T, W>(now.base + ia, x);
+      store_rounded<T, W>(now.base + ib, y);
     }
   }
 }
