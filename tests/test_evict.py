@@ -182,6 +182,25 @@ def test_twice_and_in_a_graph(pkg):
     c.check(d, (torch.arange(100, dtype=torch.int32).expand(2, 2, 100), *want[1:]))
 
 
+@pytest.mark.gpu
+def test_blocks_past_32_bit_offsets(pkg):
+    """The same batch at the end of caches of over 2^32 bytes: the same positions and the same bits."""
+    c = Case([300, 200], 70, 10, heads=4, dim=128)
+    want = c.expect()
+    blocks = c.kc.shape[0]
+    n = (1 << 32) // (4 * 128 * 16 * 2) + 64
+    d = c.device()
+    for k in ("kc", "vc", "wc"):
+        t = torch.empty((n,) + tuple(d[k].shape[1:]), dtype=d[k].dtype, device="cuda")
+        t[n - blocks:] = d[k]
+        d[k] = t
+    d["tables"] = torch.where(d["tables"] >= 0, d["tables"] + (n - blocks), d["tables"])
+    c.call(pkg, d)
+    for k in ("kc", "vc", "wc"):
+        d[k] = d[k][n - blocks:].contiguous()
+    c.check(d, want)
+
+
 def test_c_entry_refuses_without_a_gpu(pkg):
     c = pkg._capi
     p = ctypes.c_void_p(4096)

@@ -155,6 +155,7 @@ SHAPES = [
     ([150, 260], [50, 7], 8, 1),              # 400 rows: several workgroups
     ([20, 129], [17, 1], 3, 1),
     ([0, 17, 0], [0, 2, 0], 2, 2),
+    ([500, 333], [300, 333], 4, 2),           # the next stretch of a prompt, and a whole one
 ]
 
 
@@ -214,6 +215,51 @@ def test_rising_logits(pkg):
             c.kc[int(c.tables[0, b])] *= 1.0 + b
         c.keys[0] = torch.cat([(c.keys[0][16 * b:16 * b + 16] * (1.0 + b)) for b in range(-(-700 // 16))])
         run(pkg, c)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("masked", [True, False])
+def test_a_long_chain_over_a_long_context(pkg, masked):
+    """Many rows and many partitions: positions behind a workgroup's last row are left out of a chain."""
+    run(pkg, Case([2100], [700], 2, 2, masked=masked, dtype=torch.bfloat16))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("drafted", [[3], [40]])
+@pytest.mark.parametrize("scale", [1e9, -1e9])
+def test_logits_far_beyond_the_slack(pkg, dtype, drafted, scale):
+    """Logits of 10^10, whose last bit is worth hundreds: the softmax picks one position where the gap to the next is
+    more than the logits' own error (e of the file's head), and is finite everywhere."""
+    c = Case([300], drafted, 4, 2, dtype=dtype, masked=False, scale=scale)
+    out = c.attend(pkg, c.device())[:drafted[0]].double().cpu().numpy()
+    assert np.isfinite(out).all()
+    q, sure = c.query.double().numpy(), 0
+    for t in range(drafted[0]):
+        n = 300 - drafted[0] + t + 1
+        for h in range(4):
+            k, v = c.keys[0][:n, h // 2].double().numpy(), c.values[0][:n, h // 2].double().numpy()
+            s = scale * (k @ q[t, h])
+            e = ((c.dim + 4) * U * abs(scale) * (np.abs(k) @ np.abs(q[t, h])) + 4 * U * np.abs(s)).max()
+            order = np.argsort(-s)
+            if s[order[0]] - s[order[1]] > 2 * e + 100:
+                sure += 1
+                assert (np.abs(out[t, h] - v[order[0]]) <= 4 * HALF[dtype] * np.abs(v[order[0]]) + 2.0 ** -24).all()
+    assert sure > 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_logits_at_the_type_s_end(pkg, dtype):
+    """All logits near -10^36: no row passes for one that sees nothing."""
+    c = Case([40], [2], 2, 1, dtype=dtype, masked=False, scale=1.0)
+    c.kc[:] = torch.where(torch.isnan(c.kc), c.kc, torch.full_like(c.kc, -1e18))
+    c.q_store[:] = 1.5e16
+    out = c.attend(pkg, c.device())[:2].double().cpu().numpy()
+    for t in range(2):
+        want = c.values[0][:39 + t].double().mean(0).numpy()  # equal logits: the mean
+        for h in range(2):
+            assert (np.abs(out[t, h] - want[0]) <= 2.0 ** -6 * np.abs(c.values[0].double().numpy()).max()).all()
 
 
 @pytest.mark.gpu
@@ -418,6 +464,30 @@ def test_two_graphs_replayed_in_turn(pkg):
         for d, w in zip(devs, want):
             assert torch.equal(d["out"], w)
         assert torch.equal(devs[1]["weights"], weights)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("drafted", [[1, 1], [5, 9], [40, 33]])
+def test_blocks_past_32_bit_offsets(pkg, drafted):
+    """The same batch at the start of a small cache and at the end of one of over 2^32 bytes: the same bits."""
+    c = Case([130, 75], drafted, 4, 4, dim=128, block=16, masked=False)
+    small = c.device()
+    blocks = c.kc.shape[0]
+    n = (1 << 32) // (4 * 128 * 16 * 2) + 64          # blocks of 16 KiB: offsets past 2^32 bytes
+    big = dict(small)
+    for k in ("kc", "vc"):
+        t = torch.empty((n,) + tuple(small[k].shape[1:]), dtype=small[k].dtype, device="cuda")
+        t[n - blocks:] = small[k]
+        big[k] = t
+    big["tables"] = torch.where(small["tables"] < blocks, small["tables"] + (n - blocks), small["tables"])
+    for call in ((c.attend, c.accumulate) if max(drafted) < 10 else (c.attend,)):
+        outs = []
+        for d, total in ((small, blocks), (big, n)):
+            d["weights"] = torch.zeros(total, 4, 16, device="cuda")
+            d["out"] = torch.zeros_like(d["out"])
+            outs.append(call(pkg, d).clone())
+        assert torch.equal(outs[0], outs[1])
+        assert torch.equal(small["weights"], big["weights"][n - blocks:])
 
 
 def test_c_entry_refuses_without_a_gpu(pkg):

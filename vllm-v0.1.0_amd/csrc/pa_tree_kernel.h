@@ -32,7 +32,7 @@ namespace tree {
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
-constexpr float kNoMax = -1e30f;   // below every logit, and finite: exp2(-inf - kNoMax) = 0
+constexpr float kNoMax = -3.402823466e38f;  // below every logit, and finite: exp2(-inf - kNoMax) = 0
 constexpr float kMaxSlack = 8.f;   // how far a logit may exceed the running maximum
 
 struct F16 {
@@ -155,6 +155,26 @@ __device__ __forceinline__ Item tree_item(const TreeArgs& a) {
   return r;
 }
 
+// The steps of a partition, and those at its start that all of a workgroup's rows see: in a chain a row sees up
+// to itself, so later positions are left out (not where every row's logits are kept) and earlier ones are open.
+struct Span { int steps, open_steps; };
+template <bool KEEP>
+__device__ __forceinline__ Span tree_span(const TreeArgs& a, const TreeSeq& sq, int row0, int rows, int p0, int p1, int step) {
+  const int shared = sq.ctx - sq.queries;
+  int end = p1, open = shared;
+  if (a.mask == nullptr) {
+    const int last = (row0 + rows < sq.rows ? row0 + rows : sq.rows) - 1;
+    const int reach = shared + last / a.group + 1;
+    if (!KEEP && reach < end) end = reach;
+    open = shared + row0 / a.group + 1;
+  }
+  Span r;
+  r.steps = end > p0 ? (end - p0 + step - 1) / step : 0;
+  r.open_steps = open > p0 ? (open - p0) / step : 0;
+  if (r.open_steps > r.steps) r.open_steps = r.steps;
+  return r;
+}
+
 // The rows of a sequence whose arguments contradict each other
 template <typename E, int D>
 __device__ __forceinline__ void fill_nan(const TreeArgs& a, const TreeSeq& sq, int head) {
@@ -174,6 +194,7 @@ struct Rows {
   u32x4 qf[RT][KS];
   f32x4 o[RT][NJ], l[RT];
   float m[RT], lx[RT];
+  bool huge;  // some row's maximum is past 2^24 (the same for the whole wave)
   int query[RT], row[RT];
   bool valid[RT];
 
@@ -181,6 +202,7 @@ struct Rows {
   __device__ __forceinline__ void init(const TreeArgs& a, const TreeSeq& sq, int head, int row0, int lane) {
     const int n = lane & 15, g = lane >> 4;
     const bool aligned = ((reinterpret_cast<uintptr_t>(a.q) | (uintptr_t)(a.q_stride * (int64_t)sizeof(T))) & 15u) == 0;
+    huge = false;
     const T* qp[RT];
 #pragma unroll
     for (int t = 0; t < RT; t++) {
@@ -265,8 +287,11 @@ struct Rows {
     }
   }
 
-  // Raises the running maxima where a logit exceeds one by its slack
-  __device__ __forceinline__ void raise(const TreeArgs& a, const f32x4 (*s)[NA]) {
+  // Raises the running maxima where a logit exceeds one by its slack.  A weight is then exp2(s * scale.c - scale.m)
+  // with one rounding, of the difference; past 2^24 the product's own would show, and past 2^31 overflow: there the
+  // logits are made differences first, of rounded products.
+  struct Scale { float c, m[RT]; };
+  __device__ __forceinline__ Scale raise(const TreeArgs& a, f32x4 (*s)[NA]) {
     float top[RT];
     bool over = false;
 #pragma unroll
@@ -277,27 +302,49 @@ struct Rows {
       top[t] *= a.c;
       over |= top[t] > m[t] + (E::kBias + kMaxSlack);
     }
-    if (__builtin_amdgcn_ballot_w64(over) == 0) return;
+    Scale r;
+    r.c = a.c;
+    if (__builtin_amdgcn_ballot_w64(over) != 0) {
+      bool big = false;
 #pragma unroll
-    for (int t = 0; t < RT; t++) {
-      float high = fmaxf(m[t], top[t] - E::kBias);
-      high = fmaxf(high, __shfl_xor(high, 16));
-      high = fmaxf(high, __shfl_xor(high, 32));
-      const float f = __builtin_amdgcn_exp2f(m[t] - high);
-      m[t] = high;
-      lx[t] *= f;
-      l[t] *= f;
+      for (int t = 0; t < RT; t++) {
+        float high = fmaxf(m[t], top[t] - E::kBias);
+        high = fmaxf(high, __shfl_xor(high, 16));
+        high = fmaxf(high, __shfl_xor(high, 32));
+        const float f = __builtin_amdgcn_exp2f(m[t] - high);
+        m[t] = high;
+        lx[t] *= f;
+        l[t] *= f;
 #pragma unroll
-      for (int j = 0; j < NJ; j++) o[t][j] *= f;
+        for (int j = 0; j < NJ; j++) o[t][j] *= f;
+        big |= fabsf(high) > 0x1p24f && high != kNoMax;
+      }
+      huge = __builtin_amdgcn_ballot_w64(big) != 0;
     }
+#pragma unroll
+    for (int t = 0; t < RT; t++) r.m[t] = m[t];
+    if (huge) {
+#pragma unroll
+      for (int t = 0; t < RT; t++) {
+#pragma unroll
+        for (int i = 0; i < PT; i++) {
+          float x = s[t][i >> 2][i & 3] * a.c;
+          asm("" : "+v"(x));  // rounded before the difference
+          s[t][i >> 2][i & 3] = x - m[t];
+        }
+        r.m[t] = 0.f;
+      }
+      r.c = 1.f;
+    }
+    return r;
   }
 
   // Logits to rounded weights, and their sum; EXACT: the sum before the rounding too
   template <bool EXACT>
-  __device__ __forceinline__ u32x4 weigh(const TreeArgs& a, int t, const f32x4* s) {
+  __device__ __forceinline__ u32x4 weigh(const Scale& scale, int t, const f32x4* s) {
     float x[PT];
 #pragma unroll
-    for (int i = 0; i < PT; i++) x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i >> 2][i & 3], a.c, -m[t]));
+    for (int i = 0; i < PT; i++) x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i >> 2][i & 3], scale.c, -scale.m[t]));
     if (EXACT) {
 #pragma unroll
       for (int i = 0; i < PT; i++) lx[t] += x[i];
@@ -407,8 +454,8 @@ __global__ void __launch_bounds__(256, (RT == 1 ? 3 : 2)) pa_tree_few_kernel(con
   const int n = lane & 15, g = lane >> 4;
   const int p0 = it.part * sq.part_len;
   const int p1 = it.part == sq.parts - 1 ? sq.ctx : p0 + sq.part_len;
-  const int steps = (p1 - p0 + TS - 1) / TS;
-  const int open = sq.ctx - sq.queries - p0, open_steps = open < 0 ? 0 : (open / TS < steps ? open / TS : steps);  // seen by all rows
+  const Span span = tree_span<ACC>(a, sq, row0, ROWS, p0, p1, TS);
+  const int steps = span.steps, open_steps = span.open_steps;
   R r;
   __shared__ float sm_m[WK][ROWS], sm_l[WK][ROWS], sm_x[WK][ROWS];
   constexpr int ST = D + 4;  // rows of LDS start 4 banks apart
@@ -491,19 +538,19 @@ __global__ void __launch_bounds__(256, (RT == 1 ? 3 : 2)) pa_tree_few_kernel(con
       if (more) load_k(next.k, step + WK);
       __builtin_amdgcn_sched_barrier(0);
       if (masked) r.hide(a, sq, s, seen, tok, g);
-      r.raise(a, s);
-      u32x4 pf[RT];
+      if (ACC) {
 #pragma unroll
-      for (int t = 0; t < RT; t++) {
-        if (ACC) {
+        for (int t = 0; t < RT; t++)
           if (r.valid[t]) {
 #pragma unroll
             for (int i = 0; i < NA; i++)
               *reinterpret_cast<f32x4*>(sm + (t * 16 + n) * logit_row + step * TS + vtok + 4 * i) = s[t][i] * a.c;
           }
-        }
-        pf[t] = r.template weigh<ACC>(a, t, s[t]);
       }
+      const typename R::Scale scale = r.raise(a, s);
+      u32x4 pf[RT];
+#pragma unroll
+      for (int t = 0; t < RT; t++) pf[t] = r.template weigh<ACC>(scale, t, s[t]);
       if (masked) r.clean(sq, vf, pf, tok, g);
 #pragma unroll
       for (int t = 0; t < RT; t++)
@@ -527,17 +574,17 @@ __global__ void __launch_bounds__(256, (RT == 1 ? 3 : 2)) pa_tree_few_kernel(con
     for (int t = 0; t < RT; t++) sm_m[wk][t * 16 + n] = r.m[t];
   }
   __syncthreads();
-  float scale[RT];
+  float share[RT];
 #pragma unroll
   for (int t = 0; t < RT; t++) {
     const int row = t * 16 + n;
     float high = sm_m[0][row];
 #pragma unroll
     for (int w = 1; w < WK; w++) high = fmaxf(high, sm_m[w][row]);
-    scale[t] = any_bad ? __builtin_nanf("") : __builtin_amdgcn_exp2f(r.m[t] - high);
+    share[t] = any_bad ? __builtin_nanf("") : __builtin_amdgcn_exp2f(r.m[t] - high);
     if (g == 0) {
-      sm_l[wk][row] = r.l[t][0] * scale[t];
-      sm_x[wk][row] = r.lx[t] * scale[t];
+      sm_l[wk][row] = r.l[t][0] * share[t];
+      sm_x[wk][row] = r.lx[t] * share[t];
     }
   }
   if (ACC) {
@@ -573,7 +620,7 @@ __global__ void __launch_bounds__(256, (RT == 1 ? 3 : 2)) pa_tree_few_kernel(con
 #pragma unroll
   for (int t = 0; t < RT; t++)
 #pragma unroll
-    for (int j = 0; j < NJ; j++) *reinterpret_cast<f32x4*>(&sm_o[wk][t * 16 + n][16 * j + 4 * g]) = r.o[t][j] * scale[t];
+    for (int j = 0; j < NJ; j++) *reinterpret_cast<f32x4*>(&sm_o[wk][t * 16 + n][16 * j + 4 * g]) = r.o[t][j] * share[t];
   __syncthreads();
   for (int i = tid; i < ROWS * (D / 4); i += 256) {
     const int row = i / (D / 4), d = (i - row * (D / 4)) * 4;
@@ -619,8 +666,8 @@ __global__ void __launch_bounds__(NW * 64, 2) pa_tree_many_kernel(const TreeArgs
   const int bits = a.block_bits, B = 1 << bits;
   const int p0 = it.part * sq.part_len;
   const int p1 = it.part == sq.parts - 1 ? sq.ctx : p0 + sq.part_len;
-  const int steps = (p1 - p0 + TS - 1) / TS;
-  const int open = sq.ctx - sq.queries - p0, open_steps = open < 0 ? 0 : (open / TS < steps ? open / TS : steps);  // seen by all rows
+  const Span span = tree_span<false>(a, sq, row0, ROWS, p0, p1, TS);
+  const int steps = span.steps, open_steps = span.open_steps;
   const bool has_rows = row0 + wave * 16 * RT < sq.rows;
   if (tid == 0) sm_bad = 0;
 
@@ -702,7 +749,7 @@ __global__ void __launch_bounds__(NW * 64, 2) pa_tree_many_kernel(const TreeArgs
   // A step past the last is the last again.  Keys run one step ahead of values: when step i's turn comes its
   // logits are there, and the products of step i + 1's keys have no part in what is made of them, so the
   // matrix and the vector units work side by side in every wave.
-  const auto clamp = [&](int step) { return step < steps ? step : steps - 1; };
+  const auto clamp = [&](int step) { return step < steps ? step : (steps > 0 ? steps - 1 : 0); };
   u32x4 k_held[2][FK], v_held[2][FV];  // step i's pieces pass through set i % 2; no copies, which would wait for the loads
   f32x4 s[RT][NA];
   {
@@ -742,14 +789,14 @@ __global__ void __launch_bounds__(NW * 64, 2) pa_tree_many_kernel(const TreeArgs
       take(k, sm_k[1 - kOdd]);  // on their way while the maxima are looked at
       __builtin_amdgcn_sched_barrier(0);
       if (kMasked) r.hide(a, sq, s, seen, tok, g);
-      r.raise(a, s);
+      const typename R::Scale scale = r.raise(a, s);
       f32x4 ahead[RT][NA];
       multiply(ahead, k);
 #pragma unroll
       for (int j = 0; j < NJ; j++) v[j] = sm_v[kOdd][j * 64 + lane];
       u32x4 pf[RT];
 #pragma unroll
-      for (int t = 0; t < RT; t++) pf[t] = r.template weigh<false>(a, t, s[t]);
+      for (int t = 0; t < RT; t++) pf[t] = r.template weigh<false>(scale, t, s[t]);
       if (kMasked) r.clean(sq, v, pf, tok, g);
 #pragma unroll
       for (int j = 0; j < NJ; j++)
