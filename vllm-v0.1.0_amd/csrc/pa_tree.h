@@ -7,6 +7,7 @@
 namespace pa {
 
 constexpr int kPartTokens = 128;  // a context partition is a multiple of this: a step for each of 4 waves
+constexpr int kTreeSorted = 256;  // at most so many sequences are put in order by a workgroup: one to a thread
 
 struct TreeArgs {
   void* out;                // [num_tokens, num_heads, head_size]
@@ -30,6 +31,7 @@ struct TreeArgs {
   int parts, part_len;      // at most so many context partitions, of at most part_len positions
   int row_tiles;            // workgroups along a sequence's rows
   int form;                 // TreeForm
+  bool sorted;              // whether sequences are taken by falling context length
 };
 
 // What a launch does with one sequence, the same for every kernel that asks.
@@ -76,18 +78,18 @@ __device__ __forceinline__ void add_weights(const TreeArgs& a, const TreeSeq& sq
   *reinterpret_cast<f32x4*>(to) = w;
 }
 
-// LDS of the few-rows kernel where logits are kept: 48 KiB (three workgroups to a CU), or what joining its
-// waves takes
+// LDS of the few-rows kernel where logits are kept: 76 KiB, what two workgroups to a CU leave each other, or what
+// joining its waves takes.  A context that fits is weighed without a second kernel and without its logits' way
+// through memory: 96 sequences of up to 4096 tokens, 4 rows, 182 us; 227 us with 48 KiB and parts of 1408 tokens,
+// although three workgroups share a CU then (even lengths of 2560 tokens, which fit either: 175 us both).
 constexpr int tree_logit_floats(int head_size, int row_tiles) {
   const int join = 4 * 16 * row_tiles * (head_size + 4);
-  return join > 12288 ? join : 12288;
+  return join > 19456 ? join : 19456;
 }
 
 // The kernel for a launch of at most `rows` rows a sequence and kv head, by the rows of a workgroup.
 enum TreeForm { kTreeFew16 = 16, kTreeFew32 = 32, kTreeMany64 = 64, kTreeMany128 = 128 };
 inline TreeForm tree_form(int64_t rows, bool accumulate, bool fp32) {
-  const int forced = tuning_int("PA_TREE_FORM", 0);
-  if (forced > 0) return static_cast<TreeForm>(forced);
   if (rows <= 16) return kTreeFew16;
   if (rows <= 32 || accumulate) return kTreeFew32;  // only the few-rows kernel keeps its logits
   if (rows <= 64 || fp32) return kTreeMany64;  // fp32 queries of two tiles a wave do not fit its registers

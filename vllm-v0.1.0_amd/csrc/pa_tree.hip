@@ -116,7 +116,7 @@ struct TreePlan {
 
 constexpr int kChipCUs = 256;
 constexpr int kMaxParts = 64;
-constexpr int kSplitTokens = 1408;
+constexpr int kMinPart = 256;
 
 TreePlan tree_plan(int num_seqs, int num_heads, int num_kv_heads, int head_size, int max_ctx, int max_query, bool accumulate,
                    bool fp32) {
@@ -125,19 +125,22 @@ TreePlan tree_plan(int num_seqs, int num_heads, int num_kv_heads, int head_size,
   const int rows = tree_form(p.max_rows, accumulate, fp32);
   p.row_tiles = (int)std::max<int64_t>(1, (p.max_rows + rows - 1) / rows);
   const int64_t groups = std::max<int64_t>(1, (int64_t)num_seqs * num_kv_heads * p.row_tiles);
-  // Partitions until there are three workgroups to a CU, none shorter than two steps of every wave.
-  const int64_t want = tuning_int("PA_TREE_WANT", 2 * kChipCUs) / groups;
-  const int min_part = tuning_int("PA_TREE_MIN_PART", 256);
-  const int64_t most = std::max<int64_t>(1, (max_ctx + min_part - 1) / min_part);
+  // As many partitions as two workgroups to a CU allow: those are resident at once, and one more would wait for
+  // them (8 sequences of up to 4096 tokens, trees of 64, 8 kv heads of 32: 55 us; for one workgroup to a CU 70,
+  // for three 68).  None is shorter than two steps of every wave (one sequence of 1024 tokens, 26 drafted, 32
+  // heads: 13.5 us; with parts of 128 14.4, of 512 15.9).
+  const int64_t want = 2 * kChipCUs / groups;
+  const int64_t most = std::max<int64_t>(1, (max_ctx + kMinPart - 1) / kMinPart);
   const int64_t parts = std::max<int64_t>(1, std::min<int64_t>({want, most, (int64_t)kMaxParts}));
   int64_t len = (max_ctx + parts - 1) / parts;
-  len = std::max<int64_t>(kPartTokens, (len + kPartTokens - 1) / kPartTokens * kPartTokens);
   if (accumulate) {  // a row's logits and 4 floats behind them, for every row of a workgroup
     const int64_t room = (tree_logit_floats(head_size, rows / 16) / std::min<int64_t>(rows, p.max_rows) - 4) / kPartTokens * kPartTokens;
-    // A context that does not fit has to go out in parts: shorter ones then, which balance a ragged batch better
-    // (96 sequences of up to 4096 tokens, 8 kv heads: parts of 3072 257 us, of 1408 224, of 768 223).
-    if (len > room) len = std::min<int64_t>(room, kSplitTokens);
+    if (len > room) {
+      const int64_t n = (max_ctx + room - 1) / room;
+      len = (max_ctx + n - 1) / n;
+    }
   }
+  len = std::max<int64_t>(kPartTokens, (len + kPartTokens - 1) / kPartTokens * kPartTokens);
   p.part_len = (int)len;
   p.parts = (int)std::max<int64_t>(1, ((int64_t)max_ctx + p.part_len - 1) / p.part_len);
   p.tile_rows = rows;
@@ -230,6 +233,9 @@ int tree_entry(const char* what, void* out, const void* query, const void* key_c
   a.part_len = p.part_len;
   a.row_tiles = p.row_tiles;
   a.form = p.tile_rows;
+  // Where workgroups wait for a CU, the longest go first (24 sequences of up to 4096 tokens, trees of 64, 8 kv
+  // heads of 32: 113 us, as they come 131; where all lengths are alike the sort costs 1 %).
+  a.sorted = num_seqs > 1 && num_seqs <= kTreeSorted && items * p.row_tiles > kChipCUs;
   hipStream_t st = static_cast<hipStream_t>(stream);
   int rc;
   switch (dtype) {

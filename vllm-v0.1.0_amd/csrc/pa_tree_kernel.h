@@ -136,6 +136,16 @@ __device__ __forceinline__ void lds_barrier() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
+// Until the last product's result can be read (8 and 10 instructions' time).  Before a branch that the results are
+// used behind: where a short way and a long one meet again, the compiler was seen to count its waits along the long
+// one alone, and along the short one the first element read was an old one.
+template <typename E> __device__ __forceinline__ void settle() {
+  __builtin_amdgcn_sched_barrier(0);
+  if (sizeof(typename E::storage) == 4) asm volatile("s_nop 9");
+  else asm volatile("s_nop 7");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
 // The workgroup's item.  Workgroups that share a (sequence, partition, head) share an XCD and its L2;
 // the groups go round the XCDs.
 struct Item {
@@ -173,6 +183,29 @@ __device__ __forceinline__ Span tree_span(const TreeArgs& a, const TreeSeq& sq, 
   r.open_steps = open > p0 ? (open - p0) / step : 0;
   if (r.open_steps > r.steps) r.open_steps = r.steps;
   return r;
+}
+
+// The sequence that stands `place`-th by falling context length, those alike in their order.  Workgroups are dealt
+// out in the order of their items: with the longest first, a CU that is done early takes up a shorter one, and no
+// long one is left to run alone at the end.
+__device__ __forceinline__ int by_length(const TreeArgs& a, int place, int* len, int* found) {
+  const int t = threadIdx.x, n = a.num_seqs;
+  const int mine = t < n ? a.ctx[t] : -2147483647 - 1;
+  len[t] = mine;
+  __syncthreads();
+  int before = 0;
+  if (t < n) {
+    for (int j = 0; j < n; j += 4) {
+      const int4 o = *reinterpret_cast<const int4*>(len + j);
+      before += (o.x > mine) | ((o.x == mine) & (j < t)) ? 1 : 0;
+      before += (o.y > mine) | ((o.y == mine) & (j + 1 < t)) ? 1 : 0;
+      before += (o.z > mine) | ((o.z == mine) & (j + 2 < t)) ? 1 : 0;
+      before += (o.w > mine) | ((o.w == mine) & (j + 3 < t)) ? 1 : 0;
+    }
+    if (before == place) *found = t;
+  }
+  __syncthreads();
+  return __builtin_amdgcn_readfirstlane(*found);
 }
 
 // The rows of a sequence whose arguments contradict each other
@@ -437,12 +470,17 @@ __device__ __forceinline__ void store_row(const TreeArgs& a, const TreeSeq& sq, 
 // kernel that joins partitions.  Written out step by step, with the loop's reads, they cost three times as much
 // (96 sequences of up to 4096 tokens, 4 query heads to a kv head: 48 us of 247, for 31 MB).
 template <typename E, int D, int B, int RT, bool ACC>
-__global__ void __launch_bounds__(256, (RT == 1 ? 3 : 2)) pa_tree_few_kernel(const TreeArgs a) {
+__global__ void __launch_bounds__(256, (RT == 1 && !ACC ? 3 : 2)) pa_tree_few_kernel(const TreeArgs a) {
   typedef typename E::storage T;
   typedef Rows<E, D, RT> R;
   constexpr int X = R::X, TS = R::TS, KS = R::KS, NA = R::NA, NJ = R::NJ, PT = R::PT, WK = 4, ROWS = 16 * RT;
-  const Item it = tree_item(a);
+  Item it = tree_item(a);
   if (!it.exists) return;
+  if (a.sorted) {
+    __shared__ __attribute__((aligned(16))) int sm_len[kTreeSorted];
+    __shared__ int sm_found;
+    it.seq = by_length(a, it.seq, sm_len, &sm_found);
+  }
   const TreeSeq sq = tree_seq(a, it.seq);
   const int tid = threadIdx.x, lane = tid & 63, wk = __builtin_amdgcn_readfirstlane(tid >> 6);
   if (sq.bad) {
@@ -535,6 +573,7 @@ __global__ void __launch_bounds__(256, (RT == 1 ? 3 : 2)) pa_tree_few_kernel(con
       // the table entries two steps ahead go out before the next keys: waiting for them waits for nothing else
       const Ids after = load_ids(step + 2 * WK < steps ? step + 2 * WK : step);
       __builtin_amdgcn_sched_barrier(0);  // the loads where they stand: earlier, they would take registers twice
+      if (!kInner) settle<E>();
       if (more) load_k(next.k, step + WK);
       __builtin_amdgcn_sched_barrier(0);
       if (masked) r.hide(a, sq, s, seen, tok, g);
@@ -644,16 +683,22 @@ __global__ void __launch_bounds__(256, (RT == 1 ? 3 : 2)) pa_tree_few_kernel(con
 // products take them (a lane's 16 bytes at 16 * lane: no bank conflicts); wave w fetches pieces w, w + NW, ...
 // from the caches at the addresses that the few-rows kernel would use.  Two buffers of each kind, filled from
 // registers that were loaded two turns before; one barrier a step.
-template <typename E, int D, int RT, int NW>
-__global__ void __launch_bounds__(NW * 64, 2) pa_tree_many_kernel(const TreeArgs a) {
+template <typename E, int D, int RT>
+__global__ void __launch_bounds__(256, 2) pa_tree_many_kernel(const TreeArgs a) {
+  constexpr int NW = 4;
   typedef typename E::storage T;
   typedef Rows<E, D, RT> R;
   constexpr int X = R::X, TS = R::TS, KS = R::KS, NA = R::NA, NJ = R::NJ, PT = R::PT, ROWS = 16 * RT * NW;
   constexpr int NK = NA * KS, FK = (NK + NW - 1) / NW, FV = (NJ + NW - 1) / NW;
   __shared__ __attribute__((aligned(16))) u32x4 sm_k[2][NK * 64], sm_v[2][NJ * 64];
   __shared__ int sm_bad;
-  const Item it = tree_item(a);
+  Item it = tree_item(a);
   if (!it.exists) return;
+  if (a.sorted) {
+    __shared__ __attribute__((aligned(16))) int sm_len[kTreeSorted];
+    __shared__ int sm_found;
+    it.seq = by_length(a, it.seq, sm_len, &sm_found);
+  }
   const TreeSeq sq = tree_seq(a, it.seq);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   if (sq.bad) {
@@ -848,9 +893,10 @@ static void tree_few(const TreeArgs& a, int form, unsigned grid, hipStream_t st)
 template <typename E, int D>
 static void tree_pick_form(const TreeArgs& a, unsigned grid, hipStream_t st) {
   const int form = a.form;
-  if (form == kTreeMany64) hipLaunchKernelGGL((pa_tree_many_kernel<E, D, 1, 4>), dim3(grid), dim3(256), 0, st, a);
-  else if (form == kTreeMany128) hipLaunchKernelGGL((pa_tree_many_kernel<E, D, (E::kX == 8 ? 2 : 1), 4>), dim3(grid), dim3(256), 0, st, a);
-  else {
+  if (form == kTreeMany64) hipLaunchKernelGGL((pa_tree_many_kernel<E, D, 1>), dim3(grid), dim3(256), 0, st, a);
+  else if (form == kTreeMany128) {
+    if constexpr (E::kX == 8) hipLaunchKernelGGL((pa_tree_many_kernel<E, D, 2>), dim3(grid), dim3(256), 0, st, a);
+  } else {
     if (a.block_bits == 3) tree_few<E, D, 8>(a, form, grid, st);
     else if (a.block_bits == 4) tree_few<E, D, 16>(a, form, grid, st);
     else tree_few<E, D, 32>(a, form, grid, st);
