@@ -267,7 +267,8 @@ int pa_append_single_query_cached_kv_attention(
  * max_context_len and max_query_len bound the sequences' own and size the launch.  A
  * sequence that exceeds one, has more new tokens than context or more context
  * than its table, or whose table names a block >= num_blocks, gets NaN in its
- * rows; nothing outside the given arrays is read or written for it.
+ * rows; nothing outside the given arrays is read or written for it.  With
+ * max_query_len 0 no sequence has new tokens, and nothing is done.
  *
  * workspace: pa_tree_workspace_bytes(...) bytes of device memory (0: none),
  * 16-byte aligned, contents irrelevant; two calls that may overlap in time need
@@ -301,8 +302,9 @@ int pa_tree_cached_kv_attention(
  * weights (the caller zeroes those).  Blocks must not be shared by two sequences
  * of the call, as their sums would race.  Contexts too long to be read by one
  * workgroup keep their logits in the workspace: num_seqs * num_heads *
- * max_query_len * max_context_len * 4 bytes.  The sums are made
- * in one order, whatever the timing.
+ * max_query_len * max_context_len * 4 bytes.  The sums are made in one order,
+ * whatever the timing.  Sequences that contradict the call leave the weights
+ * alone; one with a block outside the cache gets NaN for them, too.
  */
 int pa_cached_kv_attention_accumulate(
     void* out, const void* query, const void* key_cache, const void* value_cache,

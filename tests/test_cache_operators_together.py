@@ -47,6 +47,16 @@ def test_keep_path_refuses_paths_that_do_not_rise(pkg):
         keep_path([], [], torch.zeros(1, 1, dtype=torch.int32), [0], [[2, 1]])
 
 
+def test_keep_path_refuses_what_is_not_in_the_tables(pkg):
+    """On the host: an index that is not there would end a program on the GPU."""
+    from vllm_amd.worker import keep_path
+    keys, values = [torch.zeros(4, 1, 8, 16, 8).half()], [torch.zeros(4, 1, 64, 16).half()]
+    tables = torch.zeros(1, 2, dtype=torch.int32)
+    for first, paths in (([30], [[0, 2]]), ([-1], [[1]]), ([0, 0], [[0], [1]]), ([], [[1]])):
+        with pytest.raises(ValueError, match="block table"):
+            keep_path(keys, values, tables, first, paths)
+
+
 @pytest.mark.parametrize("scaling", ["none", "linear", "ntk", "yarn"])
 def test_cos_sin_cache_against_its_definition(pkg, scaling):
     """Angles by hand in float64; a float32 table rounds cos and sin once (2^-24 of an amplitude below 1.2)."""

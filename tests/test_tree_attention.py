@@ -186,6 +186,34 @@ def test_long_contexts_in_partitions(pkg, dim, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("seqs,kv,most", [(40, 8, 3), (37, 8, 20), (256, 2, 3), (257, 1, 2)])
+def test_batches_of_more_workgroups_than_the_chip(pkg, seqs, kv, most):
+    """Sequences of all lengths, equal and empty ones among them: up to 256 of them are taken by their length."""
+    drafted = [i * 7 % (most + 1) for i in range(seqs)]
+    lens = [max(t, i * 37 % 90 if i % 5 else 41) for i, t in enumerate(drafted)]
+    for masked in (True, False):
+        c = Case(lens, drafted, 2 * kv, kv, masked=masked, seed=seqs)
+        oracle = c.oracle()
+        d = c.device()
+        c.check_out(c.attend(pkg, d), oracle)
+    d = c.device()
+    d["weights"] = torch.zeros(c.kc.shape[0], kv, 16, device="cuda")
+    c.check_out(c.accumulate(pkg, d), oracle)
+    got = d["weights"].double().cpu().numpy()
+    for i, n in enumerate(lens):
+        for pos in range(n if drafted[i] else 0):
+            w = got[int(c.tables[i, pos // 16]), :, pos % 16]
+            assert (np.abs(w - oracle[2][i][:, pos]) <= oracle[3][i][:, pos] + U * oracle[2][i][:, pos] + 1e-30).all()
+    # one that contradicts itself in their midst: its own rows only
+    d["lens_t"][20] = 10 ** 6
+    out = c.accumulate(pkg, d)
+    wrong = torch.zeros(sum(drafted), dtype=torch.bool)
+    wrong[int(c.starts[20]):int(c.starts[21])] = True
+    assert torch.equal(torch.isnan(out[:sum(drafted)]).flatten(1).all(1).cpu(), wrong)
+    assert torch.equal(torch.isnan(out[:sum(drafted)]).flatten(1).any(1).cpu(), wrong)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("parts_ctx", [16384, 12289])
 def test_more_partitions_than_half_a_wave(pkg, parts_ctx):
     run(pkg, Case([parts_ctx], [1], 1, 1, dim=64))
@@ -433,6 +461,20 @@ def test_accumulate_skips_contradictory_sequences(pkg):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("length", [60, 9000])
+def test_a_bad_block_spoils_its_sequence_s_weights_alone(pkg, length):
+    c = Case([length, 70], [1, 1], 2, 2, masked=False)
+    d = c.device()
+    d["weights"] = torch.ones(c.kc.shape[0], 2, 16, device="cuda")
+    d["tables"][0, 1] = 2 ** 31 - 1
+    c.accumulate(pkg, d)
+    assert bool(torch.isnan(d["out"][0]).all()) and bool(torch.isfinite(d["out"][1]).all())
+    w = d["weights"]
+    assert bool(torch.isnan(w[int(c.tables[0, 0])]).all()) and bool((w[int(c.tables[0, 1])] == 1).all())
+    assert bool((w[int(c.tables[1, 0])] >= 1).all())
+
+
+@pytest.mark.gpu
 def test_two_graphs_replayed_in_turn(pkg):
     """Two captured calls of other sizes, replayed on a stream of their own with eager calls between."""
     cases = [Case([700, 33], [5, 3], 4, 2, seed=1), Case([90, 1200], [1, 1], 2, 1, masked=False, seed=2)]
@@ -515,6 +557,7 @@ def test_c_entry_refuses_without_a_gpu(pkg):
         assert call(acc, kc=ctypes.c_void_p(4104)) == c.PA_ERR_INVALID_ARGUMENT and "aligned" in c.last_error()
         assert call(acc, scale=math.inf) == c.PA_ERR_INVALID_ARGUMENT and "finite" in c.last_error()
         assert call(acc, scale=math.nan) == c.PA_ERR_INVALID_ARGUMENT
+        assert call(acc, scale=-3e38) == c.PA_ERR_INVALID_ARGUMENT and "finite" in c.last_error()  # times log2(e) it is not
         assert call(acc, st=200) == c.PA_ERR_INVALID_ARGUMENT and "shorter" in c.last_error()
         assert call(acc, mc=65) == c.PA_ERR_INVALID_ARGUMENT and "cannot hold" in c.last_error()
         assert call(acc, mq=65) == c.PA_ERR_INVALID_ARGUMENT and "exceeds" in c.last_error()

@@ -177,7 +177,7 @@ int tree_entry(const char* what, void* out, const void* query, const void* key_c
              "%s: null pointer argument", what);
   PA_REQUIRE(aligned16(out) && aligned16(key_cache) && aligned16(value_cache) && aligned16(weight_cache),
              "%s: out and the caches must be 16-byte aligned", what);
-  PA_REQUIRE(isfinite(scale), "%s: scale must be finite", what);
+  PA_REQUIRE(isfinite(scale * 1.44269504088896340736f), "%s: scale must be finite, its product with log2(e) too", what);
   PA_REQUIRE(num_tokens == 1 || q_stride >= (int64_t)num_heads * head_size, "%s: query row stride is shorter than a token row", what);
   PA_REQUIRE((int64_t)max_num_blocks_per_seq * block_size >= max_context_len,
              "%s: block tables of %d blocks cannot hold max_context_len %d", what, max_num_blocks_per_seq, max_context_len);

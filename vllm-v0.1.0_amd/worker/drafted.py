@@ -38,6 +38,8 @@ def keep_path(key_caches: List[torch.Tensor], value_caches: List[torch.Tensor], 
     Tokens already in place are not touched; the moves of one layer are one gather and one scatter."""
     if cache_ops is None:
         from .. import cache_ops  # HIP module; no fallback
+    if len(paths) > block_tables.shape[0] or len(paths) > len(first_positions):
+        raise ValueError(f"{len(paths)} paths for a block table of {block_tables.shape[0]} sequences, {len(first_positions)} positions")
     sequence, source, target = [], [], []
     for s, path in enumerate(paths):
         for i, t in enumerate(path):
@@ -49,9 +51,11 @@ def keep_path(key_caches: List[torch.Tensor], value_caches: List[torch.Tensor], 
                 target.append(first_positions[s] + i)
     if not sequence:
         return
+    block = value_caches[0].shape[3]
+    if min(target) < 0 or max(source) >= block_tables.shape[1] * block:
+        raise ValueError(f"a path runs from position {min(target)} to {max(source)}, the block tables hold {block_tables.shape[1] * block}")
     device = block_tables.device
     seq, src, dst = (torch.tensor(x, dtype=torch.int64, device=device) for x in (sequence, source, target))
-    block = value_caches[0].shape[3]
     slots = [(block_tables[seq, at // block].long() * block + at % block).int() for at in (src, dst)]
     heads, dim = value_caches[0].shape[1:3]
     key = torch.empty(len(sequence), heads, dim, dtype=value_caches[0].dtype, device=device)
