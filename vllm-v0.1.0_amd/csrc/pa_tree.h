@@ -31,7 +31,7 @@ struct TreeArgs {
   int parts, part_len;      // at most so many context partitions, of at most part_len positions
   int row_tiles;            // workgroups along a sequence's rows
   int form;                 // TreeForm
-  bool sorted;              // whether sequences are taken by falling context length
+  bool sorted;              // whether sequences are taken by falling length of their partitions
 };
 
 // What a launch does with one sequence, the same for every kernel that asks.
@@ -39,6 +39,12 @@ struct TreeSeq {
   int first, queries, rows, ctx, parts, part_len;
   bool bad;  // the arguments contradict each other: its rows are filled with NaN
 };
+
+// As few partitions as part_len allows, of one length: a last one of any length would leave others waiting.
+__device__ __forceinline__ int tree_part_len(const TreeArgs& a, int ctx) {
+  const int p = (int)(((int64_t)ctx + a.part_len - 1) / a.part_len);
+  return (int)(((int64_t)ctx + p - 1) / p + kPartTokens - 1) / kPartTokens * kPartTokens;
+}
 
 __device__ __forceinline__ TreeSeq tree_seq(const TreeArgs& a, int s) {
   TreeSeq r;
@@ -50,10 +56,8 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeArgs& a, int s) {
   r.bad = lo < 0 || hi > a.num_tokens || hi < lo || r.queries > a.max_query || r.ctx < r.queries || r.ctx > a.max_ctx ||
           r.ctx > ((int64_t)a.table_width << a.block_bits);
   r.rows = r.queries * a.group;
-  // as few partitions as part_len allows, of one length: a last one of any length would leave others waiting
   const int ctx = r.bad || r.ctx < 1 ? 1 : r.ctx;
-  const int p = (ctx + a.part_len - 1) / a.part_len;
-  r.part_len = ((ctx + p - 1) / p + kPartTokens - 1) / kPartTokens * kPartTokens;
+  r.part_len = tree_part_len(a, ctx);
   r.parts = (ctx + r.part_len - 1) / r.part_len;
   return r;
 }

