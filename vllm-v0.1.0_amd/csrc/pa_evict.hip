@@ -29,6 +29,8 @@
 // 32 sequences of 8 kv heads of 128, 16 bits, of 8192 positions to 2048, random weights: 23 us to select, 309 to
 // move, 4.3 TB/s of the lines that it touches.  A walk over the old positions, each sent to its slot, took 40 % longer:
 // the slots have to be counted along the way, and its loads wait for conditional stores.
+#include <type_traits>
+
 #include "pa_common.h"
 
 namespace pa {
@@ -224,6 +226,7 @@ __global__ void __launch_bounds__(kThreads) pa_evict_select_kernel(const EvictAr
 }
 
 constexpr int kSlots = 16;  // a wave's step
+constexpr int kRows = 16;   // and its rows of the values
 
 // X: elements of 16 bytes
 template <typename T, int X>
@@ -325,12 +328,15 @@ pa_evict_move_kernel(const EvictArgs a, const int32_t* __restrict__ tables, cons
     return;
   }
 
-  constexpr int VECS = kSlots / X, U = 64 / kSlots;
-  const int first_slot = (lane & (VECS - 1)) * X, row = (kind - a.key_tasks) * (64 / VECS) + lane / VECS;
-  const bool mine = row < a.head_size;
-  char* base = vc + (int64_t)head * a.tile_bytes + (int64_t)(mine ? row : 0) * B * (int)sizeof(T);
+  // Values: a slot and four rows to a load, so that its 64 elements lie in few lines: a block's four rows are one or
+  // two.  With a lane to a row and eight slots the address units were what it waited for (87 % busy, 297 us).
+  constexpr int U = 64 / kSlots, G = 2, LOADS = kRows / 4;
+  const int t = lane & (kSlots - 1), sub = lane / kSlots, row0 = (kind - a.key_tasks) * kRows;
+  const int row_bytes = B * (int)sizeof(T);
+  char* base = vc + (int64_t)head * a.tile_bytes + (int64_t)(row0 + sub) * row_bytes;
   const auto address = [&](int slot) { return base + (int64_t)(slot >> bits) * block_bytes + (slot & (B - 1)) * (int)sizeof(T); };
-  constexpr int G = 2;
+  // four rows are all within the head or none: the head size is a multiple of X
+  const auto rows = [&](int k) { return row0 + 4 * k < a.head_size ? 4 * k * row_bytes : 0; };
   Page page[G];
   int next[G];
 #pragma unroll
@@ -339,16 +345,17 @@ pa_evict_move_kernel(const EvictArgs a, const int32_t* __restrict__ tables, cons
     next[q] = ask(w0 + 64 * (G + q));
   }
   for (int w = w0; w <= last; w += 64 * G) {
-    T v[G][U][X];
+    T v[G][U][LOADS];
     char* dst[G][U];
 #pragma unroll
     for (int q = 0; q < G; q++) {
       const int from = source(page[q]), to = target(page[q], w + 64 * q);
 #pragma unroll
       for (int u = 0; u < U; u++) {
+        const char* src = address(lane_of(from, u * kSlots + t));
 #pragma unroll
-        for (int i = 0; i < X; i++) v[q][u][i] = *reinterpret_cast<const T*>(address(lane_of(from, u * kSlots + first_slot + i)));
-        dst[q][u] = address(lane_of(to, u * kSlots + first_slot));
+        for (int k = 0; k < LOADS; k++) v[q][u][k] = *reinterpret_cast<const T*>(src + rows(k));
+        dst[q][u] = address(lane_of(to, u * kSlots + t));
       }
     }
     Page ahead[G];
@@ -356,23 +363,46 @@ pa_evict_move_kernel(const EvictArgs a, const int32_t* __restrict__ tables, cons
     for (int q = 0; q < G; q++) ahead[q] = look_up(next[q], w + 64 * (G + q));
 #pragma unroll
     for (int q = 0; q < G; q++) next[q] = ask(w + 64 * (2 * G + q));
+    const auto put = [&](auto whole) {
+      constexpr bool kWhole = decltype(whole)::value;  // all slots within the budget, all rows within the head
 #pragma unroll
-    for (int q = 0; q < G; q++)
+      for (int q = 0; q < G; q++)
 #pragma unroll
-      for (int u = 0; u < U; u++) {
-        const int left = last + 1 - (w + 64 * q + kSlots * u + first_slot);  // slots of this lane within the budget
-        if (mine && left >= X) {
-          u32x4 r;
+        for (int u = 0; u < U; u++) {
+          const int slot = w + 64 * q + kSlots * u + t;
+          if constexpr (X == 4) {
 #pragma unroll
-          for (int i = 0; i < 4; i++)
-            r[i] = X == 4 ? (uint32_t)v[q][u][i] : (uint32_t)v[q][u][(2 * i) % X] | (uint32_t)v[q][u][(2 * i + 1) % X] << 16;
-          *reinterpret_cast<u32x4*>(dst[q][u]) = r;
-        } else if (mine && left > 0) {  // the slots behind the budget stay as they are
+            for (int k = 0; k < LOADS; k++)
+              if (kWhole || (slot <= last && row0 + 4 * k < a.head_size)) *reinterpret_cast<T*>(dst[q][u] + 4 * k * row_bytes) = v[q][u][k];
+          } else {
+            const int mine = t & 3, quad = slot - mine;  // of four lanes' slots and four loads' rows a lane stores its row
+            char* to = dst[q][u] + 4 * mine * row_bytes - (kWhole || slot <= last ? slot - quad : last - quad) * (int)sizeof(T);
 #pragma unroll
-          for (int i = 0; i < X; i++)
-            if (i < left) reinterpret_cast<T*>(dst[q][u])[i] = v[q][u][i];
+            for (int k = 0; k < LOADS; k += 4) {
+              uint32_t pair[2], r[2];
+#pragma unroll
+              for (int i = 0; i < 2; i++) {
+                const uint32_t x = v[q][u][k + 2 * i], y = v[q][u][k + 2 * i + 1];
+                const uint32_t other = (uint32_t)__builtin_amdgcn_mov_dpp((int)(mine & 1 ? x : y), 0xb1, 0xf, 0xf, true);
+                pair[i] = mine & 1 ? other | y << 16 : x | other << 16;
+              }
+              const uint32_t other = (uint32_t)__builtin_amdgcn_mov_dpp((int)(mine & 2 ? pair[0] : pair[1]), 0x4e, 0xf, 0xf, true);
+              r[0] = mine & 2 ? other : pair[0];
+              r[1] = mine & 2 ? pair[1] : other;
+              const bool in = row0 + 4 * (k + mine) < a.head_size;
+              if (kWhole || (in && quad + 3 <= last)) {
+                *reinterpret_cast<uint2*>(to + 4 * k * row_bytes) = make_uint2(r[0], r[1]);
+              } else if (in) {  // the slots behind the budget stay as they are
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                  if (quad + i <= last) reinterpret_cast<T*>(to + 4 * k * row_bytes)[i] = (T)(r[i >> 1] >> (16 * (i & 1)));
+              }
+            }
+          }
         }
-      }
+    };
+    if (w + 64 * G - 1 <= last && row0 + kRows <= a.head_size) put(std::true_type{});
+    else put(std::false_type{});
 #pragma unroll
     for (int q = 0; q < G; q++) page[q] = ahead[q];
   }
@@ -436,7 +466,7 @@ extern "C" int pa_evict_cached_kv(void* key_cache, void* value_cache, float* wei
   a.head_size = head_size;
   a.tile_bytes = head_size * block_size * elem_size(dtype);
   a.key_tasks = (head_size / x + 3) / 4;
-  a.value_tasks = (head_size + 4 * x - 1) / (4 * x);  // 64 / (16 / x) rows each
+  a.value_tasks = (head_size + kRows - 1) / kRows;
   a.tasks = cells * (a.key_tasks + a.value_tasks + 1);
   PA_REQUIRE(cells <= 0x7fffffff && (a.tasks + 3) / 4 <= 0x7fffffff, "%s: too many heads for one launch", what);
   hipStream_t st = static_cast<hipStream_t>(stream);
