@@ -17,18 +17,18 @@
 // weights are held in LDS with their part of the block table, and moved from
 // there; longer contexts read the rest from L2 in every pass.
 //
-// pa_evict_move_kernel: one wave to 4 chunks of the keys of a (sequence, kv head), or as many rows of the values as
-// have 64 pieces of 16 bytes in 16 slots.  It walks the slots from the first that changes, and takes each from where
-// the list says: a slot comes from a position at or behind it, so what later slots need is never overwritten, and
-// waves never share a byte.  A key's piece is one load and one store; a value's is put together of single elements,
-// as positions lie side by side in a row.  128 slots' loads are on their way at once, the block table's for the next
-// 128 and the list's for the ones behind them too.  Bound by HBM: with a quarter of the positions kept at random
-// every 128-byte line of the old blocks holds one that stays, so the whole of them is read (the values' rows of a
-// block even with one position in sixteen).
+// pa_evict_move_kernel: one wave to 4 chunks of the keys of a (sequence, kv head), or to 16 rows of its values.  It
+// walks the slots from the first that changes, and takes each from where the list says: a slot comes from a position at
+// or behind it, so what later slots need is never overwritten, and waves never share a byte.  A key's piece is one
+// load and one store; a value's is put together of single elements, as positions lie side by side in a row.  128 slots'
+// loads are on their way at once, the block table's for the next 128 and the list's for the ones behind them too.
+// Bound by HBM: with a quarter of the positions kept at random nearly every 128-byte line of the old blocks holds one
+// that stays, so the whole of them is read (the values' rows of a block even with one position in sixteen).
 //
-// 32 sequences of 8 kv heads of 128, 16 bits, of 8192 positions to 2048, random weights: 23 us to select, 309 to
-// move, 4.3 TB/s of the lines that it touches.  A walk over the old positions, each sent to its slot, took 40 % longer:
-// the slots have to be counted along the way, and its loads wait for conditional stores.
+// 32 sequences of 8 kv heads of 128, 16 bits, of 8192 positions to 2048, random weights: 23 us to select, 279 to
+// move, 1.27 GB by the counters = 4.5 TB/s.  With 32 rows to a wave 300 (and 8 sequences of 16000 to 4000 236 in all
+// against 182: too few waves), with 2 or 1 chunks of the keys no less.  A walk over the old positions, each sent to its
+// slot, took 40 % longer: the slots have to be counted along the way, and its loads wait for conditional stores.
 #include <type_traits>
 
 #include "pa_common.h"
@@ -329,7 +329,8 @@ pa_evict_move_kernel(const EvictArgs a, const int32_t* __restrict__ tables, cons
   }
 
   // Values: a slot and four rows to a load, so that its 64 elements lie in few lines: a block's four rows are one or
-  // two.  With a lane to a row and eight slots the address units were what it waited for (87 % busy, 297 us).
+  // two.  16-bit elements are exchanged among four lanes, which store four slots each: a batch that has been through
+  // it before, 59 us; a lane to a row and eight slots of it, 64 rows' lines to a load, 71.
   constexpr int U = 64 / kSlots, G = 2, LOADS = kRows / 4;
   const int t = lane & (kSlots - 1), sub = lane / kSlots, row0 = (kind - a.key_tasks) * kRows;
   const int row_bytes = B * (int)sizeof(T);
