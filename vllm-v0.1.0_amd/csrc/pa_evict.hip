@@ -25,9 +25,11 @@
 // Bound by HBM: with a quarter of the positions kept at random nearly every 128-byte line of the old blocks holds one
 // that stays, so the whole of them is read (the values' rows of a block even with one position in sixteen).
 //
-// 32 sequences of 8 kv heads of 128, 16 bits, of 8192 positions to 2048, random weights: 23 us to select, 279 to
-// move, 1.27 GB by the counters = 4.5 TB/s.  With 32 rows to a wave 300 (and 8 sequences of 16000 to 4000 236 in all
-// against 182: too few waves), with 2 or 1 chunks of the keys no less.  A walk over the old positions, each sent to its
+// A wave is a workgroup: a gather keeps a CU's address unit for its 64 elements, and waves of one workgroup share
+// one (a sequence of 8192 positions to 2048 in all 48 us, four waves to a workgroup 70; 32 sequences 290 and 315).
+// 32 sequences of 8 kv heads of 128, 16 bits, of 8192 positions to 2048, random weights: 23 us to select, 255 to
+// move, 1.27 GB by the counters = 5.0 TB/s.  With 32 rows to a wave instead of 16, 7 % more (and 8 sequences of
+// 16000 to 4000 236 in all against 182: too few waves), with 2 or 1 chunks of the keys no less.  A walk over the old positions, each sent to its
 // slot, took 40 % longer: the slots have to be counted along the way, and its loads wait for conditional stores.
 #include <type_traits>
 
@@ -46,7 +48,6 @@ struct EvictArgs {
   int heads, head_size, block_bits, num_blocks, table_width, max_ctx, budget, recent;
   int tile_bytes;           // of one head's share of a block: head_size * block * element size
   int key_tasks, value_tasks;  // waves of a (sequence, head): for its keys, for its values, and one for its weights
-  int64_t tasks;
 };
 
 namespace {
@@ -230,15 +231,14 @@ constexpr int kRows = 16;   // and its rows of the values
 
 // X: elements of 16 bytes
 template <typename T, int X>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(64)
 pa_evict_move_kernel(const EvictArgs a, const int32_t* __restrict__ tables, const int32_t* __restrict__ all_kept,
                      const int32_t* __restrict__ firsts, char* __restrict__ kc, char* __restrict__ vc,
                      float* __restrict__ weights) {
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t task = (int64_t)blockIdx.x * 4 + wave;
-  if (task >= a.tasks) return;
+  const int lane = threadIdx.x;
+  const unsigned task = blockIdx.x;
   const int kinds = a.key_tasks + a.value_tasks + 1;
-  const int sh = (int)(task / kinds), kind = (int)(task - (int64_t)sh * kinds);
+  const int sh = (int)(task / (unsigned)kinds), kind = (int)(task - (unsigned)sh * (unsigned)kinds);
   const int first = firsts[sh];
   if (first < 0) return;
   const int seq = sh / a.heads, head = sh - seq * a.heads;
@@ -330,7 +330,7 @@ pa_evict_move_kernel(const EvictArgs a, const int32_t* __restrict__ tables, cons
 
   // Values: a slot and four rows to a load, so that its 64 elements lie in few lines: a block's four rows are one or
   // two.  16-bit elements are exchanged among four lanes, which store four slots each: a batch that has been through
-  // it before, 59 us; a lane to a row and eight slots of it, 64 rows' lines to a load, 71.
+  // it before, 59 us with four waves to a workgroup; a lane to a row and eight slots of it, 64 rows' lines to a load, 71.
   constexpr int U = 64 / kSlots, G = 2, LOADS = kRows / 4;
   const int t = lane & (kSlots - 1), sub = lane / kSlots, row0 = (kind - a.key_tasks) * kRows;
   const int row_bytes = B * (int)sizeof(T);
@@ -468,17 +468,17 @@ extern "C" int pa_evict_cached_kv(void* key_cache, void* value_cache, float* wei
   a.tile_bytes = head_size * block_size * elem_size(dtype);
   a.key_tasks = (head_size / x + 3) / 4;
   a.value_tasks = (head_size + kRows - 1) / kRows;
-  a.tasks = cells * (a.key_tasks + a.value_tasks + 1);
-  PA_REQUIRE(cells <= 0x7fffffff && (a.tasks + 3) / 4 <= 0x7fffffff, "%s: too many heads for one launch", what);
+  const int64_t tasks = cells * (a.key_tasks + a.value_tasks + 1);
+  PA_REQUIRE(tasks <= 0x7fffffff, "%s: too many heads for one launch", what);
   hipStream_t st = static_cast<hipStream_t>(stream);
   hipLaunchKernelGGL(pa_evict_select_kernel, dim3((unsigned)cells), dim3(kThreads), 0, st, a);
   PA_CHECK_LAUNCH(what);
   if (max_context_len <= budget) return PA_OK;  // no sequence can lose a position
-  const dim3 grid((unsigned)((a.tasks + 3) / 4));
+  const dim3 grid((unsigned)tasks);
   if (elem_size(dtype) == 4)
-    hipLaunchKernelGGL((pa_evict_move_kernel<uint32_t, 4>), grid, dim3(256), 0, st, a, a.tables, a.kept, a.first, a.kc, a.vc, a.weights);
+    hipLaunchKernelGGL((pa_evict_move_kernel<uint32_t, 4>), grid, dim3(64), 0, st, a, a.tables, a.kept, a.first, a.kc, a.vc, a.weights);
   else
-    hipLaunchKernelGGL((pa_evict_move_kernel<uint16_t, 8>), grid, dim3(256), 0, st, a, a.tables, a.kept, a.first, a.kc, a.vc, a.weights);
+    hipLaunchKernelGGL((pa_evict_move_kernel<uint16_t, 8>), grid, dim3(64), 0, st, a, a.tables, a.kept, a.first, a.kc, a.vc, a.weights);
   PA_CHECK_LAUNCH(what);
   return PA_OK;
 }
