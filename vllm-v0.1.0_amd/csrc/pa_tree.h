@@ -82,13 +82,14 @@ __device__ __forceinline__ void add_weights(const TreeArgs& a, const TreeSeq& sq
   *reinterpret_cast<f32x4*>(to) = w;
 }
 
-// LDS of the few-rows kernel where logits are kept: 76 KiB, what two workgroups to a CU leave each other, or what
-// joining its waves takes.  A context that fits is weighed without a second kernel and without its logits' way
-// through memory: 96 sequences of up to 4096 tokens, 4 rows, 182 us; 227 us with 48 KiB and parts of 1408 tokens,
-// although three workgroups share a CU then (even lengths of 2560 tokens, which fit either: 175 us both).
-constexpr int tree_logit_floats(int head_size, int row_tiles) {
-  const int join = 4 * 16 * row_tiles * (head_size + 4);
-  return join > 19456 ? join : 19456;
+// LDS of the few-rows kernel: what joining its waves takes and, where logits are kept, the rows of a workgroup times
+// a partition's length.  They may take 76 KiB, what two workgroups to a CU leave each other: a context that fits is
+// weighed without a second kernel and without its logits' way through memory (96 sequences of up to 4096 tokens, 4
+// rows, 182 us; with 48 KiB and parts of 1408 tokens 227, although three workgroups share a CU then).
+constexpr int kTreeLogitFloats = 19456;
+constexpr int tree_few_floats(int head_size, int row_tiles, int logit_rows, int part_len) {
+  const int join = 4 * 16 * row_tiles * (head_size + 4), logits = logit_rows * (part_len + 4);
+  return join > logits ? join : logits;
 }
 
 // The kernel for a launch of at most `rows` rows a sequence and kv head, by the rows of a workgroup.

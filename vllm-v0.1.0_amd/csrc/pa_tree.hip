@@ -135,7 +135,7 @@ TreePlan tree_plan(int num_seqs, int num_heads, int num_kv_heads, int head_size,
   const int64_t parts = std::max<int64_t>(1, std::min<int64_t>({want, most, (int64_t)kMaxParts}));
   int64_t len = (max_ctx + parts - 1) / parts;
   if (accumulate) {  // a row's logits and 4 floats behind them, for every row of a workgroup
-    const int64_t room = (tree_logit_floats(head_size, rows / 16) / std::min<int64_t>(rows, p.max_rows) - 4) / kPartTokens * kPartTokens;
+    const int64_t room = (kTreeLogitFloats / std::min<int64_t>(rows, p.max_rows) - 4) / kPartTokens * kPartTokens;
     if (len > room) {
       const int64_t n = (max_ctx + room - 1) / room;
       len = (max_ctx + n - 1) / n;

@@ -477,7 +477,7 @@ __device__ __forceinline__ void store_row(const TreeArgs& a, const TreeSeq& sq, 
 // kernel that joins partitions.  Written out step by step, with the loop's reads, they cost three times as much
 // (96 sequences of up to 4096 tokens, 4 query heads to a kv head: 48 us of 247, for 31 MB).
 template <typename E, int D, int B, int RT, bool ACC>
-__global__ void __launch_bounds__(256, (RT == 1 && !ACC ? 3 : 2)) pa_tree_few_kernel(const TreeArgs a) {
+__global__ void __launch_bounds__(256, (RT == 1 ? 3 : 2)) pa_tree_few_kernel(const TreeArgs a) {
   typedef typename E::storage T;
   typedef Rows<E, D, RT> R;
   constexpr int X = R::X, TS = R::TS, KS = R::KS, NA = R::NA, NJ = R::NJ, PT = R::PT, WK = 4, ROWS = 16 * RT;
@@ -504,7 +504,7 @@ __global__ void __launch_bounds__(256, (RT == 1 && !ACC ? 3 : 2)) pa_tree_few_ke
   R r;
   __shared__ float sm_m[WK][ROWS], sm_l[WK][ROWS], sm_x[WK][ROWS];
   constexpr int ST = D + 4;  // rows of LDS start 4 banks apart
-  __shared__ __attribute__((aligned(16))) float sm[ACC ? tree_logit_floats(D, RT) : WK * ROWS * ST];
+  extern __shared__ __attribute__((aligned(16))) float sm[];  // tree_few_floats()
   const int logit_row = sq.part_len + 4;
 
   const int32_t* table = a.tables + (int64_t)it.seq * a.table_width;
@@ -891,38 +891,51 @@ __global__ void __launch_bounds__(256, 2) pa_tree_many_kernel(const TreeArgs a) 
     }
 }
 
-template <typename E, int D, int B>
-static void tree_few(const TreeArgs& a, int form, unsigned grid, hipStream_t st) {
-  if (a.weights != nullptr) {
-    if (form == kTreeFew16) hipLaunchKernelGGL((pa_tree_few_kernel<E, D, B, 1, true>), dim3(grid), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((pa_tree_few_kernel<E, D, B, 2, true>), dim3(grid), dim3(256), 0, st, a);
-  } else {
-    if (form == kTreeFew16) hipLaunchKernelGGL((pa_tree_few_kernel<E, D, B, 1, false>), dim3(grid), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((pa_tree_few_kernel<E, D, B, 2, false>), dim3(grid), dim3(256), 0, st, a);
+template <typename E, int D, int B, int RT, bool ACC>
+static int tree_few_launch(const TreeArgs& a, unsigned grid, hipStream_t st) {
+  // as much LDS as this launch's logits take: short contexts leave room for a third workgroup on a CU
+  // (108 sequences of up to 176 tokens, 16 heads of 64: 24 us, with 76 KiB for all 36)
+  const int floats = tree_few_floats(D, RT, ACC ? (a.max_rows < 16 * RT ? a.max_rows : 16 * RT) : 0, a.part_len);
+  const void* kernel = reinterpret_cast<const void*>(&pa_tree_few_kernel<E, D, B, RT, ACC>);
+  if (floats * 4 > 65536) {
+    const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, floats * 4);
+    if (e != hipSuccess) return fail(PA_ERR_HIP, "cached attention of several queries: hipFuncSetAttribute: %s", hipGetErrorString(e));
   }
+  hipLaunchKernelGGL((pa_tree_few_kernel<E, D, B, RT, ACC>), dim3(grid), dim3(256), floats * 4, st, a);
+  return PA_OK;
+}
+
+template <typename E, int D, int B>
+static int tree_few(const TreeArgs& a, int form, unsigned grid, hipStream_t st) {
+  if (a.weights != nullptr)
+    return form == kTreeFew16 ? tree_few_launch<E, D, B, 1, true>(a, grid, st) : tree_few_launch<E, D, B, 2, true>(a, grid, st);
+  return form == kTreeFew16 ? tree_few_launch<E, D, B, 1, false>(a, grid, st) : tree_few_launch<E, D, B, 2, false>(a, grid, st);
 }
 
 template <typename E, int D>
-static void tree_pick_form(const TreeArgs& a, unsigned grid, hipStream_t st) {
+static int tree_pick_form(const TreeArgs& a, unsigned grid, hipStream_t st) {
   const int form = a.form;
   if (form == kTreeMany64) hipLaunchKernelGGL((pa_tree_many_kernel<E, D, 1>), dim3(grid), dim3(256), 0, st, a);
   else if (form == kTreeMany128) {
     if constexpr (E::kX == 8) hipLaunchKernelGGL((pa_tree_many_kernel<E, D, 2>), dim3(grid), dim3(256), 0, st, a);
   } else {
-    if (a.block_bits == 3) tree_few<E, D, 8>(a, form, grid, st);
-    else if (a.block_bits == 4) tree_few<E, D, 16>(a, form, grid, st);
-    else tree_few<E, D, 32>(a, form, grid, st);
+    if (a.block_bits == 3) return tree_few<E, D, 8>(a, form, grid, st);
+    if (a.block_bits == 4) return tree_few<E, D, 16>(a, form, grid, st);
+    return tree_few<E, D, 32>(a, form, grid, st);
   }
+  return PA_OK;
 }
 
 template <typename E>
 static int tree_launch(const TreeArgs& a, int head_size, unsigned grid, hipStream_t st) {
+  int rc;
   switch (head_size) {
-    case 64: tree_pick_form<E, 64>(a, grid, st); break;
-    case 80: tree_pick_form<E, 80>(a, grid, st); break;
-    case 96: tree_pick_form<E, 96>(a, grid, st); break;
-    default: tree_pick_form<E, 128>(a, grid, st); break;
+    case 64: rc = tree_pick_form<E, 64>(a, grid, st); break;
+    case 80: rc = tree_pick_form<E, 80>(a, grid, st); break;
+    case 96: rc = tree_pick_form<E, 96>(a, grid, st); break;
+    default: rc = tree_pick_form<E, 128>(a, grid, st); break;
   }
+  if (rc != PA_OK) return rc;
   PA_CHECK_LAUNCH("cached attention of several queries");
   return PA_OK;
 }
