@@ -509,6 +509,29 @@ def test_two_graphs_replayed_in_turn(pkg):
 
 
 @pytest.mark.gpu
+def test_captured_with_the_most_logits_a_workgroup_holds(pkg):
+    """Over 64 KiB of them, weighed in the launch itself: the same bits eagerly and replayed."""
+    c = Case([4096, 4000, 9], [1, 1, 1], 8, 2, masked=False)
+    d = c.device()
+    d["weights"] = torch.zeros(c.kc.shape[0], 2, 16, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        c.accumulate(pkg, d)
+    graph.replay()
+    first = d["weights"].clone()
+    e = c.device()
+    e["weights"] = torch.zeros_like(first)
+    c.accumulate(pkg, e)
+    c.check_out(e["out"], c.oracle())
+    for _ in range(3):
+        d["weights"].zero_()
+        d["out"].fill_(7.0)
+        torch.randn(1 << 20, device="cuda").sum().item()
+        graph.replay()
+        assert torch.equal(d["out"], e["out"]) and torch.equal(d["weights"], e["weights"]) and torch.equal(first, e["weights"])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("drafted", [[1, 1], [5, 9], [40, 33]])
 def test_blocks_past_32_bit_offsets(pkg, drafted):
     """The same batch at the start of a small cache and at the end of one of over 2^32 bytes: the same bits."""
