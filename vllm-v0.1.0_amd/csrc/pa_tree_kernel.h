@@ -689,7 +689,9 @@ __global__ void __launch_bounds__(256, (RT == 1 ? 3 : 2)) pa_tree_few_kernel(con
 // NW waves of RT tiles each.  A step's operands are KS x NA + D / 16 pieces of 1 KiB, in LDS exactly as the
 // products take them (a lane's 16 bytes at 16 * lane: no bank conflicts); wave w fetches pieces w, w + NW, ...
 // from the caches at the addresses that the few-rows kernel would use.  Two buffers of each kind, filled from
-// registers that were loaded two turns before; one barrier a step.
+// registers that were loaded two turns before.  Step i's turn reads keys i + 1 and values i, and fills the other
+// buffer of each kind with keys i + 2 and values i + 1: between two barriers a buffer is either read or filled.  One
+// barrier a step keeps to that, and one more behind the reads of keys 0, which no turn makes.
 //
 // Bound by the matrix and vector units, which one wave of each SIMD feeds in turn: 32 sequences of 8192 tokens, 64
 // queries each, 8 kv heads of 32: 366 us = 750 TFLOP/s of the 1150 that a large library product reaches (matrix units
@@ -827,6 +829,7 @@ __global__ void __launch_bounds__(256, 2) pa_tree_many_kernel(const TreeArgs a) 
   {
     u32x4 k[NA][KS];
     take(k, sm_k[0]);
+    lds_barrier();  // the first turn fills this buffer anew
     multiply(s, k);
   }
   int next_k = load_ids(clamp(3)).k, next_v = load_ids(clamp(2)).v;
