@@ -651,3 +651,29 @@ def test_modules_refuse_what_does_not_fit(pkg):
         call(mc=1000)
     with pytest.raises(RuntimeError, match="exceeds"):
         call(mc=1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("heads", [2, 12, 30])                    # 10, 60 and 150 rows: each kernel
+@pytest.mark.parametrize("length", [300, 517, 600, 1030, 1200])   # 2, 3 (the draft in two of them), 3, 5 and 5 partitions
+def test_infinities_that_are_seen_come_through_every_number_of_partitions(pkg, length, heads, dtype):
+    """As test_infinities_and_nan_in_places_not_seen, where the rows' shares of the context are joined."""
+    c = Case([length], [10], heads, 2, dtype=dtype, seed=length)
+    c.mask[:] = True
+    c.mask[:6, [1, 3, 5]] = False   # rows 0..5 see none of them
+    c.mask[6, [3, 5]] = False       # row 6 sees +inf
+    c.mask[7, [1, 5]] = False       # row 7 sees -inf
+    c.mask[8, [1, 3]] = False       # row 8 sees NaN
+    c.mask[9, 5] = False            # row 9 sees both infinities
+    want, bound = c.oracle()[:2]
+    d = c.device()
+    for i, val in ((1, math.inf), (3, -math.inf), (5, math.nan)):
+        pos = length - 10 + i
+        d["vc"][int(c.tables[0, pos // 16]), :, ::2, pos % 16] = val
+    out = c.attend(pkg, d)[:10].double().cpu().numpy()
+    limit = bound + HALF[dtype] * (np.abs(want) + bound) + 2.0 ** -25
+    assert (np.abs(out[:6] - want[:6]) <= limit[:6]).all()
+    assert (np.abs(out[6:, :, 1::2] - want[6:, :, 1::2]) <= limit[6:, :, 1::2]).all()
+    assert (out[6, :, ::2] == math.inf).all() and (out[7, :, ::2] == -math.inf).all()
+    assert np.isnan(out[8:, :, ::2]).all()

@@ -47,7 +47,11 @@ __device__ __forceinline__ void join_row(const TreeArgs& a, int D, int64_t row_i
     }
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-      const float m = p + i < sq.parts ? st[i].x : -INFINITY;  // a partition past the last weighs nothing
+      // a partition past the last is the last again, and weighs nothing; its sums may be infinite, which no weight of
+      // 0 would take out
+      const bool there = p + i < sq.parts;
+      const float m = there ? st[i].x : -INFINITY;
+      v[i] = there ? v[i] : f32x4{0, 0, 0, 0};
       const float top = fmaxf(high, m);
       const float was = __builtin_amdgcn_exp2f(high - top), is = __builtin_amdgcn_exp2f(m - top);
       high = top;
