@@ -257,3 +257,14 @@ def test_module_refuses_what_does_not_fit(pkg):
     d = c.device()
     with pytest.raises(RuntimeError, match="num_recent"):
         pkg.cache_ops.evict_cached_kv(d["kc"], d["vc"], d["wc"], d["tables"], d["lens"], d["kept"], 11, 20)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("block", [8, 16, 32])
+@pytest.mark.parametrize("recent", [0, 777])
+def test_contexts_past_the_selection_s_lds_beside_shorter_ones(pkg, dtype, block, recent):
+    """Weights that are held on chip and moved at once, and weights that are read again and moved by waves of their own, in
+    one launch: three heads, sequences above, at and below the border, and one that keeps what it has."""
+    run(pkg, Case([16400, 2500, 16384, 17011, 900], 2000, recent, heads=3, dim=64, block=block, dtype=dtype, seed=block))
+    run(pkg, Case([20100, 16385], 16390, recent, heads=3, dim=8, block=block, dtype=dtype, weights="few", seed=recent))
