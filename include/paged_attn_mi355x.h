@@ -299,7 +299,8 @@ int pa_tree_cached_kv_attention(
  *
  * A sequence generating one token a step passes T = 1; after a prompt, a call
  * with its last T tokens as queries gives the earlier positions their first
- * weights (the caller zeroes those).  Blocks must not be shared by two sequences
+ * weights (the caller zeroes those, and those of accepted drafted tokens, which
+ * pa_tree_cached_kv_attention gives none).  Blocks must not be shared by two sequences
  * of the call, as their sums would race.  Contexts too long to be read by one
  * workgroup keep their logits in the workspace: num_seqs * num_heads *
  * max_query_len * max_context_len * 4 bytes.  The sums are made in one order,

@@ -282,3 +282,91 @@ def test_drafts_accepted_then_weights_then_eviction(pkg, heads, kv, interleaved)
     e.step(3)
     e.check_weights()
     e.accept([[1], [0]], *e.draft([[-1, -1], [-1, 0]]))
+
+
+class HostCacheOps:
+    """gather_cached_kv and reshape_and_cache on host tensors."""
+
+    @staticmethod
+    def gather_cached_kv(key, value, kc, vc, slots):
+        block = vc.shape[3]
+        b, o = slots.long() // block, slots.long() % block
+        key.copy_(kc[b, :, :, o].flatten(2))
+        value.copy_(vc[b, :, :, o])
+
+    @staticmethod
+    def reshape_and_cache(key, value, kc, vc, slots):
+        block = vc.shape[3]
+        b, o = slots.long() // block, slots.long() % block
+        kc[b, :, :, o] = key.unflatten(2, (kc.shape[2], kc.shape[4]))
+        vc[b, :, :, o] = value
+
+
+@pytest.mark.parametrize("paths", [[[0, 2, 6], [1, 2]], [[0, 1], []], [[], [3]], [[], []]], ids=str)
+def test_keep_path_starts_accepted_weights_from_zero(pkg, paths):
+    """Two layers: keys and values of the path move, its weights are 0 whatever their blocks held before, all others stay."""
+    from vllm_amd.worker import keep_path
+    gen = torch.Generator().manual_seed(3)
+    kv, dim, block, first = 2, 8, 4, [6, 3]
+    tables = torch.randperm(10, generator=gen).int().view(2, 5)
+    kcs = [torch.randn(10, kv, dim // 4, block, 4, generator=gen) for _ in range(2)]
+    vcs = [torch.randn(10, kv, dim, block, generator=gen) for _ in range(2)]
+    wcs = [torch.rand(10, kv, block, generator=gen) for _ in range(2)]
+    for s in range(2):
+        for pos in range(first[s], 20):
+            for w in wcs:
+                w[int(tables[s, pos // block]), :, pos % block] = math.nan
+    want = [w.clone() for w in wcs]
+    old = [v.clone() for v in vcs]
+    for s, path in enumerate(paths):
+        for i in range(len(path)):
+            for w in want:
+                w[int(tables[s, (first[s] + i) // block]), :, (first[s] + i) % block] = 0.0
+    keep_path(kcs, vcs, tables, first, paths, HostCacheOps, weight_caches=wcs)
+    for w, e in zip(wcs, want):
+        assert torch.equal(w.view(torch.int32), e.view(torch.int32))
+    for v, o in zip(vcs, old):
+        for s, path in enumerate(paths):
+            for i, t in enumerate(path):
+                to, src = first[s] + i, first[s] + t
+                assert torch.equal(v[int(tables[s, to // block]), :, :, to % block], o[int(tables[s, src // block]), :, :, src % block])
+
+
+def test_keep_path_refuses_weights_that_do_not_fit(pkg):
+    from vllm_amd.worker import keep_path
+    keys, values = [torch.zeros(4, 1, 8, 16, 8).half()], [torch.zeros(4, 1, 64, 16).half()]
+    tables = torch.zeros(1, 2, dtype=torch.int32)
+    for weights in ([], [torch.zeros(4, 1, 16)] * 2, [torch.zeros(4, 2, 16)], [torch.zeros(4, 1, 8)], [torch.zeros(3, 1, 16)]):
+        with pytest.raises(ValueError, match="weight"):
+            keep_path(keys, values, tables, [0], [[0]], HostCacheOps, weight_caches=weights)
+    # in place already, but past the table: nothing moves, weights would be written
+    with pytest.raises(ValueError, match="block table"):
+        keep_path(keys, values, tables, [31], [[0, 1]], HostCacheOps, weight_caches=[torch.zeros(4, 1, 16)])
+    with pytest.raises(ValueError, match="block table"):
+        keep_path(keys, values, tables, [-1], [[0]], HostCacheOps, weight_caches=[torch.zeros(4, 1, 16)])
+
+
+@pytest.mark.gpu
+def test_accepted_drafts_do_not_outlive_heavier_positions(pkg):
+    """The weight cache holds NaN wherever nothing was weighed, and eviction keeps NaN before all else: the entries of
+    accepted tokens have to start from 0 with the path."""
+    from vllm_amd.worker import keep_path
+    e = Engine(pkg, seed=11)
+    e.step(40)
+    paths = [[0, 2, 6], [0, 1]]
+    kn, vn, starts = e.draft([[-1, 0, 0, 1, -1, 4, 2], [-1, 0, 0]])
+    keep_path([e.kc], [e.vc], e.tables, e.lens, paths, weight_caches=[e.wc])
+    for s, path in enumerate(paths):
+        for t in path:
+            e.keys[s].append(kn[starts[s] + t])
+            e.values[s].append(vn[starts[s] + t])
+        e.lens[s] += len(path)
+        e.true[s] += len(path)
+    e.weights = [np.concatenate((w, np.zeros((e.kv, n - w.shape[1]))), 1) for w, n in zip(e.weights, e.lens)]
+    e.check_weights()
+    for _ in range(3):
+        e.step()
+    e.check_weights()
+    evict_and_rebuild(e, 30, 2)
+    e.step(2)
+    e.check_weights()

@@ -7,7 +7,7 @@ tokens move to consecutive slots, and the context ends behind them.  No counterp
 """
 from __future__ import annotations
 
-from typing import List, Sequence
+from typing import List, Optional, Sequence
 
 import numpy as np
 import torch
@@ -32,33 +32,58 @@ def tree_mask(parents: Sequence[Sequence[int]], device: torch.device | str = "cu
 
 
 def keep_path(key_caches: List[torch.Tensor], value_caches: List[torch.Tensor], block_tables: torch.Tensor,
-              first_positions: Sequence[int], paths: Sequence[Sequence[int]], cache_ops=None) -> None:
+              first_positions: Sequence[int], paths: Sequence[Sequence[int]], cache_ops=None,
+              weight_caches: Optional[List[torch.Tensor]] = None) -> None:
     """Moves every sequence's accepted drafted tokens, paths[s] (rising indices into its draft), to the
     consecutive positions from first_positions[s] on (the context length without the draft), in all layers.
-    Tokens already in place are not touched; the moves of one layer are one gather and one scatter."""
+    Tokens already in place are not touched; the moves of one layer are one gather and one scatter.
+
+    weight_caches, one per layer, where weights are accumulated for cache_ops.evict_cached_kv: the accepted
+    positions' entries start from 0.  Attention of a tree gives its tokens no weights, and an entry holds whatever
+    its block did before it was handed out, which an eviction would take for a weight."""
     if cache_ops is None:
         from .. import cache_ops  # HIP module; no fallback
     if len(paths) > block_tables.shape[0] or len(paths) > len(first_positions):
         raise ValueError(f"{len(paths)} paths for a block table of {block_tables.shape[0]} sequences, {len(first_positions)} positions")
-    sequence, source, target = [], [], []
+    if weight_caches is not None:
+        if len(weight_caches) != len(value_caches):
+            raise ValueError(f"{len(weight_caches)} weight caches for {len(value_caches)} layers")
+        for wc, vc in zip(weight_caches, value_caches):
+            if tuple(wc.shape) != (vc.shape[0], vc.shape[1], vc.shape[3]):
+                raise ValueError(f"a weight cache must be [num_blocks, num_kv_heads, block_size] like its value cache, is {list(wc.shape)}")
+    path_of, source, target = [], [], []
     for s, path in enumerate(paths):
         for i, t in enumerate(path):
             if i and t <= path[i - 1] or t < 0:
                 raise ValueError(f"the path of sequence {s} must rise: {list(path)}")
-            if t != i:
-                sequence.append(s)
-                source.append(first_positions[s] + t)
-                target.append(first_positions[s] + i)
-    if not sequence:
+            path_of.append(s)
+            source.append(first_positions[s] + t)
+            target.append(first_positions[s] + i)
+    moved = [i for i in range(len(target)) if source[i] != target[i]]
+    touched = moved if weight_caches is None else range(len(target))
+    if not touched:
         return
     block = value_caches[0].shape[3]
-    if min(target) < 0 or max(source) >= block_tables.shape[1] * block:
-        raise ValueError(f"a path runs from position {min(target)} to {max(source)}, the block tables hold {block_tables.shape[1] * block}")
+    low, high = min(target[i] for i in touched), max(source[i] for i in touched)
+    if low < 0 or high >= block_tables.shape[1] * block:
+        raise ValueError(f"a path runs from position {low} to {high}, the block tables hold {block_tables.shape[1] * block}")
     device = block_tables.device
-    seq, src, dst = (torch.tensor(x, dtype=torch.int64, device=device) for x in (sequence, source, target))
-    slots = [(block_tables[seq, at // block].long() * block + at % block).int() for at in (src, dst)]
+
+    def places(positions, which):
+        """The (block, offset) of positions[i] for i in which."""
+        seq = torch.tensor([path_of[i] for i in which], dtype=torch.int64, device=device)
+        at = torch.tensor([positions[i] for i in which], dtype=torch.int64, device=device)
+        return block_tables[seq, at // block].long(), at % block
+
+    if weight_caches is not None:
+        blocks, offsets = places(target, touched)
+        for wc in weight_caches:
+            wc[blocks, :, offsets] = 0.0
+    if not moved:
+        return
+    slots = [(b * block + o).int() for b, o in (places(source, moved), places(target, moved))]
     heads, dim = value_caches[0].shape[1:3]
-    key = torch.empty(len(sequence), heads, dim, dtype=value_caches[0].dtype, device=device)
+    key = torch.empty(len(moved), heads, dim, dtype=value_caches[0].dtype, device=device)
     value = torch.empty_like(key)
     for kc, vc in zip(key_caches, value_caches):
         cache_ops.gather_cached_kv(key, value, kc, vc, slots[0])
