@@ -691,3 +691,40 @@ def test_the_same_call_gives_the_same_bits(pkg, shape, dtype):
     for _ in range(20):
         d["out"].fill_(7.0)
         assert torch.equal(c.attend(pkg, d), first)
+
+
+@pytest.mark.gpu
+def test_bounds_past_the_tables_are_refused_before_memory_is_asked_for(pkg):
+    """The workspace goes by the bounds: these would take more than the card has."""
+    c = Case([20], [2], 2, 2)
+    d = c.device()
+    d["weights"] = torch.zeros(c.kc.shape[0], 2, 16, device="cuda")
+    for most in (1 << 27, 1 << 30, 2 ** 31 - 1):
+        before = torch.cuda.memory_reserved()
+        with pytest.raises(RuntimeError, match="cannot hold"):
+            pkg.attention_ops.cached_kv_attention_accumulate(d["out"], d["query"], d["kc"], d["vc"], d["weights"], 1.0, d["tables"],
+                                                             d["lens_t"], d["starts"], 16, most, most)
+        with pytest.raises(RuntimeError, match="cannot hold"):
+            pkg.attention_ops.tree_cached_kv_attention(d["out"], d["query"], d["kc"], d["vc"], 1.0, d["tables"], d["lens_t"],
+                                                       d["starts"], None, 16, most, most)
+        assert torch.cuda.memory_reserved() == before
+    # a call without rows: nothing to do, whatever its bounds
+    pkg.attention_ops.cached_kv_attention_accumulate(d["out"][:0], d["query"][:0], d["kc"], d["vc"], d["weights"], 1.0, d["tables"],
+                                                     d["lens_t"], d["starts"], 16, 1 << 30, 1 << 29)
+    pkg.attention_ops.tree_cached_kv_attention(d["out"], d["query"], d["kc"], d["vc"], 1.0, d["tables"][:0], d["lens_t"][:0],
+                                               d["starts"][:1], None, 16, 1 << 30, 1 << 29)
+
+
+def test_workspace_of_bounds_that_are_refused(pkg):
+    """No call takes them: no size is made up for them from sums that have overflowed."""
+    c = pkg._capi
+    for acc in (0, 1):
+        for most in ((1 << 30) + 1, 2 ** 31 - 300, 2 ** 31 - 1):
+            assert c.lib.pa_tree_workspace_bytes(1, 1, 1, 64, most, 1, acc, c.PA_DTYPE_F16) == 0
+        assert c.lib.pa_tree_workspace_bytes(2 ** 31 - 1, 1024, 1024, 64, 1 << 30, 1, acc, c.PA_DTYPE_F16) == 0
+        assert c.lib.pa_tree_workspace_bytes(1, 1024, 1, 64, 1 << 30, 1 << 30, acc, c.PA_DTYPE_F16) == 0
+    p = ctypes.c_void_p(4096)
+    for seqs, heads, query in ((2 ** 31 - 1, 1024, 1), (2 ** 31 - 1, 1024, 1 << 30), (64, 1024, 1 << 30)):
+        rc = c.lib.pa_tree_cached_kv_attention(p, p, p, p, 1.0, p, p, p, None, 0, seqs, 4, heads, 1024, 64, 8, 8, 1 << 27, 1 << 30, query,
+                                               heads * 64, c.PA_DTYPE_F16, None, 0, None)
+        assert rc == c.PA_ERR_INVALID_ARGUMENT and "too many" in c.last_error()

@@ -216,6 +216,13 @@ TreeShape check_tree_args(const char* what, const torch::Tensor& out, const torc
               what, ": key_cache shape does not match value_cache");
   TORCH_CHECK(max_context_len >= 0 && max_context_len <= INT32_MAX && max_query_len >= 0 && max_query_len <= INT32_MAX, what,
               ": max_context_len or max_query_len out of range");
+  // before the workspace, which goes by them, is asked for; a call without rows needs none, and its bounds do not matter
+  if (query.numel() > 0 && block_tables.size(0) > 0 && max_query_len > 0) {
+    TORCH_CHECK(max_context_len <= block_tables.size(1) * block_size, what, ": block tables of ", block_tables.size(1),
+                " blocks cannot hold max_context_len ", max_context_len);
+    TORCH_CHECK(max_query_len <= max_context_len, what, ": max_query_len ", max_query_len, " exceeds max_context_len ",
+                max_context_len, " (which counts the new tokens)");
+  }
   TORCH_CHECK(query.size(0) <= INT32_MAX && value_cache.size(0) <= INT32_MAX && block_tables.size(1) <= INT32_MAX &&
                   block_tables.size(0) <= INT32_MAX,
               what, ": too many tokens or blocks");
@@ -232,8 +239,9 @@ TreeShape check_tree_args(const char* what, const torch::Tensor& out, const torc
 // launches are queued (as in single_query_cached_kv_attention).
 torch::Tensor tree_workspace(const torch::Tensor& query, const TreeShape& sh, int max_context_len, int max_query_len,
                              bool accumulate, size_t* bytes) {
-  *bytes = pa_tree_workspace_bytes(sh.num_seqs, sh.num_heads, sh.num_kv_heads, sh.head_size, max_context_len, max_query_len,
-                                   accumulate, sh.dtype);
+  *bytes = sh.num_tokens == 0 ? 0
+                              : pa_tree_workspace_bytes(sh.num_seqs, sh.num_heads, sh.num_kv_heads, sh.head_size, max_context_len,
+                                                        max_query_len, accumulate, sh.dtype);
   return *bytes ? torch::empty({static_cast<int64_t>(*bytes)}, query.options().dtype(torch::kUInt8)) : torch::Tensor();
 }
 

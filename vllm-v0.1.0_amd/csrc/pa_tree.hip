@@ -122,6 +122,7 @@ struct TreePlan {
 constexpr int kChipCUs = 256;
 constexpr int kMaxParts = 64;
 constexpr int kMinPart = 256;
+constexpr int kMaxContext = 1 << 30;
 
 TreePlan tree_plan(int num_seqs, int num_heads, int num_kv_heads, int head_size, int max_ctx, int max_query, bool accumulate,
                    bool fp32) {
@@ -158,6 +159,13 @@ TreePlan tree_plan(int num_seqs, int num_heads, int num_kv_heads, int head_size,
   return p;
 }
 
+// Whether a launch of these bounds can be planned: a workgroup takes at most 128 rows of a kv head, a launch has at most
+// 2^31 workgroups, and the plan's sums stay within 64 bits below that.
+bool tree_fits(int num_seqs, int num_heads, int num_kv_heads, int max_ctx, int max_query) {
+  const int64_t cells = (int64_t)num_seqs * num_kv_heads, rows = (int64_t)max_query * (num_heads / num_kv_heads);
+  return max_ctx <= kMaxContext && cells <= 0x7fffffff && rows <= 0x7fffffff && cells * ((rows + 127) / 128) <= 0x7fffffff;
+}
+
 int tree_entry(const char* what, void* out, const void* query, const void* key_cache, const void* value_cache,
                float* weight_cache, bool accumulate, float scale, const int32_t* block_tables, const int32_t* context_lens,
                const int32_t* query_starts, const uint8_t* tree_mask, int64_t mask_stride, int num_seqs, int num_tokens,
@@ -188,10 +196,11 @@ int tree_entry(const char* what, void* out, const void* query, const void* key_c
              "%s: block tables of %d blocks cannot hold max_context_len %d", what, max_num_blocks_per_seq, max_context_len);
   PA_REQUIRE(max_query_len <= max_context_len, "%s: max_query_len %d exceeds max_context_len %d (which counts the new tokens)",
              what, max_query_len, max_context_len);
-  PA_REQUIRE(max_context_len <= (1 << 30), "%s: max_context_len %d is too large", what, max_context_len);
+  PA_REQUIRE(max_context_len <= kMaxContext, "%s: max_context_len %d is too large", what, max_context_len);
   PA_REQUIRE(tree_mask == nullptr || mask_stride >= 0, "%s: negative mask stride", what);
   PA_REQUIRE(num_blocks > 0, "%s: the caches have no blocks", what);
   PA_REQUIRE((int64_t)num_kv_heads * head_size * block_size * elem_size(dtype) <= 0x7fffffff, "%s: a block of a cache exceeds 2 GiB", what);
+  PA_REQUIRE(tree_fits(num_seqs, num_heads, num_kv_heads, max_context_len, max_query_len), "%s: too many rows for one launch", what);
   const TreePlan p = tree_plan(num_seqs, num_heads, num_kv_heads, head_size, max_context_len, max_query_len, accumulate,
                                 dtype == PA_DTYPE_F32);
   const int64_t items = (int64_t)num_seqs * num_kv_heads * p.parts;
@@ -200,7 +209,7 @@ int tree_entry(const char* what, void* out, const void* query, const void* key_c
   const int64_t join_groups = p.parts > 1 ? ((int64_t)num_seqs * max_query_len * num_heads + rows_per_group - 1) / rows_per_group : 0;
   const int chunks = (max_context_len + kChunk - 1) / kChunk;
   const int64_t join_grid = join_groups + (p.logit_bytes ? (int64_t)num_seqs * num_kv_heads * chunks : 0);
-  PA_REQUIRE(grid <= 0x7fffffff && join_grid <= 0x7fffffff && p.max_rows <= 0x7fffffff, "%s: too many rows for one launch", what);
+  PA_REQUIRE(grid <= 0x7fffffff && join_grid <= 0x7fffffff, "%s: too many rows for one launch", what);
   PA_REQUIRE(p.bytes() == 0 || (workspace && aligned16(workspace) && workspace_bytes >= p.bytes()),
              "%s: workspace of %zu bytes, 16-byte aligned, needed", what, p.bytes());
 
@@ -265,7 +274,7 @@ int tree_entry(const char* what, void* out, const void* query, const void* key_c
 extern "C" size_t pa_tree_workspace_bytes(int num_seqs, int num_heads, int num_kv_heads, int head_size, int max_context_len,
                                           int max_query_len, int accumulate, int dtype) {
   if (num_seqs <= 0 || num_heads <= 0 || num_kv_heads <= 0 || head_size <= 0 || max_context_len <= 0 || max_query_len <= 0 ||
-      num_heads % num_kv_heads != 0)
+      num_heads % num_kv_heads != 0 || !pa::tree_fits(num_seqs, num_heads, num_kv_heads, max_context_len, max_query_len))
     return 0;
   return pa::tree_plan(num_seqs, num_heads, num_kv_heads, head_size, max_context_len, max_query_len, accumulate != 0,
                        dtype == PA_DTYPE_F32)
