@@ -87,6 +87,7 @@ __device__ __forceinline__ void add_weights(const TreeArgs& a, const TreeSeq& sq
 // weighed without a second kernel and without its logits' way through memory (96 sequences of up to 4096 tokens, 4
 // rows, 182 us; with 48 KiB and parts of 1408 tokens 227, although three workgroups share a CU then).
 constexpr int kTreeLogitFloats = 19456;
+static_assert(4 * 16 * 2 * (128 + 4) <= kTreeLogitFloats, "joining the waves' largest shares takes no more than the logits may");
 constexpr int tree_few_floats(int head_size, int row_tiles, int logit_rows, int part_len) {
   const int join = 4 * 16 * row_tiles * (head_size + 4), logits = logit_rows * (part_len + 4);
   return join > logits ? join : logits;

@@ -901,7 +901,8 @@ static int tree_few_launch(const TreeArgs& a, unsigned grid, hipStream_t st) {
   const int floats = tree_few_floats(D, RT, ACC ? (a.max_rows < 16 * RT ? a.max_rows : 16 * RT) : 0, a.part_len);
   const void* kernel = reinterpret_cast<const void*>(&pa_tree_few_kernel<E, D, B, RT, ACC>);
   if (floats * 4 > 65536) {
-    const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, floats * 4);
+    // the most of any launch: two threads that set what their own take could lower it before the other's launch
+    const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kTreeLogitFloats * 4);
     if (e != hipSuccess) return fail(PA_ERR_HIP, "cached attention of several queries: hipFuncSetAttribute: %s", hipGetErrorString(e));
   }
   hipLaunchKernelGGL((pa_tree_few_kernel<E, D, B, RT, ACC>), dim3(grid), dim3(256), floats * 4, st, a);
