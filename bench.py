@@ -114,8 +114,8 @@ def pmc_traffic(kernel_substr, args):
     except (OSError, ValueError):
         return None, None
     fresh = pmc_sources_unchanged(table)
-    note = {True: "; the kernels' sources are unchanged since that pass",
-            False: "; STALE: the kernels' sources have changed since that pass",
+    note = {True: "; the kernels' sources and compile flags are unchanged since that pass",
+            False: "; STALE: the kernels' sources or compile flags have changed since that pass",
             None: ""}[fresh]
     for name, row in table.items():
         if not name.startswith("_") and kernel_substr in name:
@@ -124,16 +124,33 @@ def pmc_traffic(kernel_substr, args):
     return None, None
 
 
-def pmc_sources_unchanged(table):
-    """Whether the sources of the kernels counted in the committed PMC file are the ones in this tree
-    (the file records their hashes); None if it holds no hashes or a source cannot be read."""
+def kernel_flags_sha16(makefile=None):
+    """Hash of the flags that the kernels are compiled with (the Makefile's variables that its compile lines use)."""
     import hashlib
-    recorded = table.get("_kernel_sources_sha16")
+    if makefile is None:
+        with open(os.path.join(ROOT, "vllm-v0.1.0_amd", "csrc", "Makefile")) as f:
+            makefile = f.read()
+    flags = []
+    for line in makefile.replace("\\\n", " ").splitlines():
+        name, sep, value = line.partition("=")
+        if sep and name.strip(" :?") in ("ARCH", "NO_PACKED_F32", "HIPFLAGS", "HIPFLAGS_EXACT"):
+            flags.append(name.strip(" :?") + "=" + " ".join(value.split()))
+    return hashlib.sha256("\n".join(sorted(flags)).encode()).hexdigest()[:16]
+
+
+def pmc_sources_unchanged(table):
+    """Whether the kernels counted in the committed PMC file are the ones in this tree: built from the same sources
+    with the same flags (the file records the hashes of both); None if it lacks one or a source cannot be read."""
+    import hashlib
+    recorded, flags = table.get("_kernel_sources_sha16"), table.get("_kernel_flags_sha16")
     if not isinstance(recorded, dict) or not recorded:
         return None
     try:
-        return all(hashlib.sha256(open(os.path.join(ROOT, "vllm-v0.1.0_amd", "csrc", name), "rb").read()).hexdigest()[:16] == sha
+        same = all(hashlib.sha256(open(os.path.join(ROOT, "vllm-v0.1.0_amd", "csrc", name), "rb").read()).hexdigest()[:16] == sha
                    for name, sha in recorded.items())
+        if same and not flags:
+            return None
+        return same and flags == kernel_flags_sha16()
     except OSError:
         return None
 

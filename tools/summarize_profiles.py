@@ -16,6 +16,9 @@ import sys
 
 src, tag = sys.argv[1], sys.argv[2]
 root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+sys.path.insert(0, root)
+from bench import kernel_flags_sha16  # noqa: E402
+
 dst = os.path.join(root, "profiles")
 os.makedirs(dst, exist_ok=True)
 
@@ -53,10 +56,11 @@ for k, d in list(out.items()):
     d["read_bytes_corrected_x2"] = 2 * f
     d["write_bytes"] = w
     d["hbm_traffic_bytes_per_launch"] = 2 * f + w
-# what the counted kernels were built from: bench.py compares these with the tree it runs from and says so in its line
+# what the counted kernels were built from and with: bench.py compares these with the tree it runs from and says so in its line
 out["_kernel_sources_sha16"] = {
     name: hashlib.sha256(open(os.path.join(root, "vllm-v0.1.0_amd", "csrc", name), "rb").read()).hexdigest()[:16]
     for name in ("pa_decode.hip", "pa_cache.hip", "pa_common.h")}
+out["_kernel_flags_sha16"] = kernel_flags_sha16()
 with open(os.path.join(dst, f"{tag}_pmc_hbm_traffic.json"), "w") as g:
     json.dump(out, g, indent=1)
 shutil.copy(os.path.join(dst, f"{tag}_pmc_hbm_traffic.json"), os.path.join(dst, "pmc_hbm_traffic_latest.json"))
