@@ -728,3 +728,30 @@ def test_workspace_of_bounds_that_are_refused(pkg):
         rc = c.lib.pa_tree_cached_kv_attention(p, p, p, p, 1.0, p, p, p, None, 0, seqs, 4, heads, 1024, 64, 8, 8, 1 << 27, 1 << 30, query,
                                                heads * 64, c.PA_DTYPE_F16, None, 0, None)
         assert rc == c.PA_ERR_INVALID_ARGUMENT and "too many" in c.last_error()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("seqs,kv,most", [(40, 8, 3), (37, 8, 20), (256, 2, 3), (255, 1, 40)])
+@pytest.mark.parametrize("bound", [100, 2500])
+def test_many_sequences_as_they_come_and_by_their_length(pkg, seqs, kv, most, bound):
+    """The same batch under a tight bound of its contexts and under one that makes a launch take the longest first."""
+    drafted = [i * 11 % (most + 1) for i in range(seqs)]
+    lens = [max(t, i * 53 % 97 if i % 7 else 41) for i, t in enumerate(drafted)]
+    c = Case(lens, drafted, 2 * kv, kv, dtype=torch.bfloat16, seed=bound, extra_cols=160)
+    d = c.device()
+    c.check_out(c.attend(pkg, d, max_ctx=bound), c.oracle())
+    c.mask = None
+    oracle = c.oracle()
+    d = c.device()
+    d["weights"] = torch.zeros(c.kc.shape[0], kv, 16, device="cuda")
+    c.check_out(c.accumulate(pkg, d, max_ctx=bound), oracle)
+    got = d["weights"].double().cpu().numpy()
+    for i, n in enumerate(lens):
+        for pos in range(n if drafted[i] else 0):
+            w = got[int(c.tables[i, pos // 16]), :, pos % 16]
+            assert (np.abs(w - oracle[2][i][:, pos]) <= oracle[3][i][:, pos] + U * oracle[2][i][:, pos] + 1e-30).all()
+    d["lens_t"][20] = 10 ** 6                # its own rows only
+    out = c.accumulate(pkg, d, max_ctx=bound)
+    wrong = torch.zeros(sum(drafted), dtype=torch.bool)
+    wrong[int(c.starts[20]):int(c.starts[21])] = True
+    assert torch.equal(torch.isnan(out[:sum(drafted)]).flatten(1).any(1).cpu(), wrong)
