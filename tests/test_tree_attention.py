@@ -755,3 +755,77 @@ def test_many_sequences_as_they_come_and_by_their_length(pkg, seqs, kv, most, bo
     wrong = torch.zeros(sum(drafted), dtype=torch.bool)
     wrong[int(c.starts[20]):int(c.starts[21])] = True
     assert torch.equal(torch.isnan(out[:sum(drafted)]).flatten(1).any(1).cpu(), wrong)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("drafted", [[5, 3], [12, 40]])
+def test_masks_of_any_byte_and_stride(pkg, drafted):
+    """uint8 masks of any non-zero value, rows of a wider tensor from an odd address, and one row for all tokens."""
+    c = Case([70, 90], drafted, 4, 2, seed=9)
+    gen = torch.Generator().manual_seed(4)
+    values = torch.tensor([1, 2, 64, 128, 255], dtype=torch.uint8)[torch.randint(0, 5, c.mask.shape, generator=gen)] * c.mask
+    wide = torch.randint(0, 256, (c.mask.shape[0], c.mask.shape[1] + 13), generator=gen, dtype=torch.uint8)
+    wide[:, 7:7 + c.mask.shape[1]] = values
+    d = c.device()
+    d["mask"] = wide.cuda()[:, 7:7 + c.mask.shape[1]]
+    c.check_out(c.attend(pkg, d), c.oracle())
+    c.mask = c.mask[:1].expand(c.mask.shape[0], -1).contiguous()
+    d = c.device()
+    d["mask"] = c.mask[:1].cuda().expand(c.mask.shape[0], -1)
+    c.check_out(c.attend(pkg, d), c.oracle())
+
+
+@pytest.mark.gpu
+def test_two_threads_on_two_streams(pkg):
+    """Calls of two sizes from two host threads, on a stream each: the bits of the same calls one after the other."""
+    import threading
+    cases = [Case([4096, 300], [1, 1], 8, 2, masked=False, seed=1), Case([4600, 17, 900], [1, 1, 1], 8, 2, masked=False, seed=2)]
+    devs = [c.device() for c in cases]
+    want = []
+    for c, d in zip(cases, devs):
+        d["weights"] = torch.zeros(c.kc.shape[0], 2, 16, device="cuda")
+        c.accumulate(pkg, d)
+        want.append((d["out"].clone(), d["weights"].clone()))
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        c, d = cases[i], devs[i]
+        stream = torch.cuda.Stream()
+        try:
+            with torch.cuda.stream(stream):
+                for _ in range(30):
+                    d["weights"].zero_()
+                    d["out"].fill_(7.0)
+                    c.accumulate(pkg, d)
+                    if not (torch.equal(d["out"], want[i][0]) and torch.equal(d["weights"], want[i][1])):
+                        wrong.append(i)
+            stream.synchronize()
+        except Exception as e:
+            wrong.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("length,drafted", [(400, 300), (700, 40), (64, 5)])
+def test_a_bad_block_within_a_chain(pkg, length, drafted):
+    """The last block is not there: rows that reach it are NaN, rows before it NaN or their results."""
+    c = Case([length], [drafted], 4, 2, masked=False)
+    want, bound = c.oracle()[:2]
+    d = c.device()
+    last = (length - 1) // 16
+    d["tables"][0, last] = c.kc.shape[0]
+    out = c.attend(pkg, d)[:drafted].double().cpu().numpy()
+    reach = np.arange(drafted) + length - drafted >= last * 16
+    assert np.isnan(out[reach]).all()
+    rest = out[~reach]
+    limit = (bound + HALF[c.dtype] * (np.abs(want) + bound) + 2.0 ** -25)[~reach]
+    assert (np.isnan(rest) | (np.abs(rest - want[~reach]) <= limit)).all()
+    rows = np.isnan(rest).reshape(len(rest), -1)
+    assert (rows.all(1) | ~rows.any(1)).all()
