@@ -267,7 +267,8 @@ int pa_append_single_query_cached_kv_attention(
  * max_context_len and max_query_len bound the sequences' own and size the launch.  A
  * sequence that exceeds one, has more new tokens than context or more context
  * than its table, or whose table names a block >= num_blocks, gets NaN in its
- * rows; nothing outside the given arrays is read or written for it.  With
+ * rows (rows of a chain that end before such a block may have their results);
+ * nothing outside the given arrays is read or written for it.  With
  * max_query_len 0 no sequence has new tokens, and nothing is done.
  *
  * workspace: pa_tree_workspace_bytes(...) bytes of device memory (0: none),
@@ -369,8 +370,8 @@ int pa_gather_cached_kv(
  * max_context_len or its table, or whose table names a block outside the cache,
  * is left as it is too, all its kept_positions -1.  Blocks that the call writes
  * must not be shared: two sequences' moves would race, and a fork would lose its
- * positions (copy them first, pa_copy_blocks).  head_size: a multiple of x;
- * block sizes 8, 16, 32; all pa_dtype values.  workspace: pa_evict_workspace_bytes
+ * positions (copy them first, pa_copy_blocks).  head_size: a multiple of x, at
+ * most 4096; block sizes 8, 16, 32; all pa_dtype values.  workspace: pa_evict_workspace_bytes
  * of device memory, 16-byte aligned, contents irrelevant.
  */
 size_t pa_evict_workspace_bytes(int num_seqs, int num_kv_heads);

@@ -27,8 +27,9 @@
 //
 // A wave is a workgroup: a gather keeps a CU's address unit for its 64 elements, and waves of one workgroup share
 // one (a sequence of 8192 positions to 2048 in all 48 us, four waves to a workgroup 70; 32 sequences 290 and 315).
-// 32 sequences of 8 kv heads of 128, 16 bits, of 8192 positions to 2048, random weights: 23 us to select, 255 to
-// move, 1.27 GB by the counters = 5.0 TB/s.  With 32 rows to a wave instead of 16, 7 % more (and 8 sequences of
+// 32 sequences of 8 kv heads of 128, 16 bits, of 8192 positions to 2048, random weights: 22 us to select, 264 to
+// move, 1.28 GB by the counters = 4.8 TB/s.  Few heads of long contexts are bound by the walk itself, 128 slots at a
+// time: 2 sequences of one head, 15445 positions to 6464, 85 to 110 us.  With 32 rows to a wave instead of 16, 7 % more (and 8 sequences of
 // 16000 to 4000 236 in all against 182: too few waves), with 2 or 1 chunks of the keys no less.  A walk over the old
 // positions, each sent to its slot, took 40 % longer: the slots have to be counted along the way, and its loads wait
 // for conditional stores.

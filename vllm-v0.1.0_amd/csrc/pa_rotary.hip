@@ -16,7 +16,7 @@
 // One pass over the rows, bound by HBM for prompts (8192 tokens of 40 + 40 heads
 // of 128 with norms, fp16: 70 us = 4.9 TB/s of the 5.9 that an in-place pass over
 // plain memory reaches) and by the launch for the steps of a small batch (8 tokens
-// 2.7 us, 256 tokens with norms 3.7).  2^k lanes own a head (k such that a lane holds
+// 2.8 us, 256 tokens with norms 4.0).  2^k lanes own a head (k such that a lane holds
 // two vectors of the rotated part, and one of the rest): a head's sum of squares is
 // then k exchanges between lanes, and both elements of a pair are in one lane in both
 // layouts.  A lane keeps its table entries for all the heads of a token that it

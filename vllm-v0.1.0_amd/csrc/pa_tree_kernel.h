@@ -5,8 +5,9 @@
 //            positions ctx - T + i that mask[t][i] (or i <= t) lets t see
 //
 // The rows of a (sequence, kv head) are its T queries times the query heads that
-// share the head.  Both caches are read in the order that memory has, straight
-// into the operands of v_mfma_f32_16x16x32 (16 bit) / 16x16x4 (fp32), without LDS:
+// share the head.  Both caches are read in the order that memory has, which is
+// that of the operands of v_mfma_f32_16x16x32 (16 bit) / 16x16x4 (fp32): straight
+// into them where rows are few, through LDS as they are where all waves share a step:
 //   S^T = K . Q^T   a key block is [head_size / x][block][x], x elements = 16 bytes:
 //                   a lane's 16-byte load of (token, chunk) is its share of the A operand;
 //   O^T += V^T . P^T  a value block is [head_size][block]: a lane's 16-byte load of
@@ -14,12 +15,15 @@
 //                   accumulator, rounded to the type, is the B operand as it stands
 //                   once token 8 (m / 4) + 4 a + m % 4 sits in row m of the a-th of
 //                   two products (16 bit; fp32 needs no such order).
-// A row's running maximum is raised only when a logit exceeds it by 2^8 (the
-// weights then reach 2^8, which fp32 sums and both 16-bit types hold), so that
-// lanes exchange nothing in the common step: l and O keep to one scale anyway.
-// The sum of the weights is a product with a row of ones: it adds up what the
-// rounded weights really were.  fp16 weights carry a factor 2^6, so that one of
-// 2^-20 of the row's largest still has all its bits.
+// A row's running maximum is raised only when a logit, in base 2, exceeds it by 8,
+// so that lanes exchange nothing in the common step: l and O keep to one scale
+// anyway.  Weights then reach 2^8, and in fp16, where they carry a factor 2^6 so
+// that one of 2^-20 of the row's largest still has all its bits, 2^14 of the 65504
+// that the type holds.  They are rounded to the type, as a matrix product takes
+// operands of one type: off by half a step each, out by at most that of sum p |v|
+// and of itself (seen: 0.0003 in fp16 and 0.0023 in bf16 of the outputs' size, with
+// weights of fp32 0.0002 and 0.0017).  The sum of the weights is a product with a
+// row of ones: it adds up what the rounded weights really were.
 #pragma once
 
 #include <type_traits>
@@ -694,9 +698,10 @@ __global__ void __launch_bounds__(256, (RT == 1 ? 3 : 2)) pa_tree_few_kernel(con
 // barrier a step keeps to that, and one more behind the reads of keys 0, which no turn makes.
 //
 // Bound by the matrix and vector units, which one wave of each SIMD feeds in turn: 32 sequences of 8192 tokens, 64
-// queries each, 8 kv heads of 32: 366 us = 750 TFLOP/s of the 1150 that a large library product reaches (matrix units
+// queries each, 8 kv heads of 32: 348 us = 790 TFLOP/s of the 1150 that a large library product reaches (matrix units
 // 41 % busy, vector units 47 %); with a quarter of the rows, 200 us, HBM at 5.4 TB/s.  All 256 rows of a head in one
-// workgroup halve the reads from L2, but leave fewer workgroups to balance (24 ragged trees of 64: 141 us against 126).
+// workgroup halve the reads from L2, but leave fewer workgroups to balance (24 ragged trees of 64, before the longest
+// went first: 141 us against 126).
 template <typename E, int D, int RT>
 __global__ void __launch_bounds__(256, 2) pa_tree_many_kernel(const TreeArgs a) {
   constexpr int NW = 4;
@@ -897,7 +902,7 @@ __global__ void __launch_bounds__(256, 2) pa_tree_many_kernel(const TreeArgs a) 
 template <typename E, int D, int B, int RT, bool ACC>
 static int tree_few_launch(const TreeArgs& a, unsigned grid, hipStream_t st) {
   // as much LDS as this launch's logits take: short contexts leave room for a third workgroup on a CU
-  // (108 sequences of up to 176 tokens, 16 heads of 64: 24 us, with 76 KiB for all 36)
+  // (108 sequences of up to 176 tokens, 16 heads of 64: 16.4 us, with 76 KiB for all 22.3)
   const int floats = tree_few_floats(D, RT, ACC ? (a.max_rows < 16 * RT ? a.max_rows : 16 * RT) : 0, a.part_len);
   const void* kernel = reinterpret_cast<const void*>(&pa_tree_few_kernel<E, D, B, RT, ACC>);
   if (floats * 4 > 65536) {
