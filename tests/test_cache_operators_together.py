@@ -370,3 +370,17 @@ def test_accepted_drafts_do_not_outlive_heavier_positions(pkg):
     evict_and_rebuild(e, 30, 2)
     e.step(2)
     e.check_weights()
+
+
+def test_rotary_module_keeps_its_table_where_weights_are_emptied(pkg):
+    """A model that is made without memory first, then given empty memory and its checkpoint: the table is in none."""
+    from vllm_amd.layers import RotaryEmbedding, rotary_cos_sin_cache
+    want = rotary_cos_sin_cache(32, 128)
+    with torch.device("meta"):
+        m = RotaryEmbedding(64, 32, 128, qk_norm=True)
+    assert m.query_weight.is_meta
+    m = m.to_empty(device="cpu")
+    assert not m.query_weight.is_meta and "cos_sin_cache" not in m.state_dict()
+    assert torch.equal(m.cos_sin_cache, want)
+    assert torch.equal(RotaryEmbedding(64, 32, 128).to_empty(device="cpu").double().cos_sin_cache, want)
+    assert torch.equal(RotaryEmbedding(64, 32, 128, qk_norm=True).to("meta").to_empty(device="cpu").cos_sin_cache, want)

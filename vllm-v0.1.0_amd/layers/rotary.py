@@ -78,11 +78,12 @@ class RotaryEmbedding(nn.Module):
         self.key_weight = nn.Parameter(torch.ones(head_size)) if qk_norm else None
 
     def _apply(self, fn, recurse=True):
-        # .half() and .to(dtype) are meant for the weights: the table keeps its type and follows the device
+        # .half(), .to(dtype) and .to_empty() are meant for the weights, which a checkpoint fills: the table keeps its
+        # numbers, and follows the device to where they can be
         table = self.cos_sin_cache
         super()._apply(fn, recurse)
-        if self.cos_sin_cache.dtype != torch.float32:
-            self.cos_sin_cache = table.to(self.cos_sin_cache.device)
+        device = self.cos_sin_cache.device
+        self.cos_sin_cache = table if device.type == "meta" else table.to(device)
         return self
 
     def forward(self, positions: torch.Tensor, query: torch.Tensor, key: torch.Tensor) -> None:
