@@ -51,39 +51,31 @@ def keep_path(key_caches: List[torch.Tensor], value_caches: List[torch.Tensor], 
         for wc, vc in zip(weight_caches, value_caches):
             if tuple(wc.shape) != (vc.shape[0], vc.shape[1], vc.shape[3]):
                 raise ValueError(f"a weight cache must be [num_blocks, num_kv_heads, block_size] like its value cache, is {list(wc.shape)}")
-    path_of, source, target = [], [], []
+    moved, in_place = [], []  # (sequence, from, to)
     for s, path in enumerate(paths):
         for i, t in enumerate(path):
             if i and t <= path[i - 1] or t < 0:
                 raise ValueError(f"the path of sequence {s} must rise: {list(path)}")
-            path_of.append(s)
-            source.append(first_positions[s] + t)
-            target.append(first_positions[s] + i)
-    moved = [i for i in range(len(target)) if source[i] != target[i]]
-    touched = moved if weight_caches is None else range(len(target))
+            (in_place if t == i else moved).append((s, first_positions[s] + t, first_positions[s] + i))
+    touched = moved if weight_caches is None else moved + in_place
     if not touched:
         return
     block = value_caches[0].shape[3]
-    low, high = min(target[i] for i in touched), max(source[i] for i in touched)
+    low, high = min(to for _, _, to in touched), max(at for _, at, _ in touched)
     if low < 0 or high >= block_tables.shape[1] * block:
         raise ValueError(f"a path runs from position {low} to {high}, the block tables hold {block_tables.shape[1] * block}")
     device = block_tables.device
-
-    def places(positions, which):
-        """The (block, offset) of positions[i] for i in which."""
-        seq = torch.tensor([path_of[i] for i in which], dtype=torch.int64, device=device)
-        at = torch.tensor([positions[i] for i in which], dtype=torch.int64, device=device)
-        return block_tables[seq, at // block].long(), at % block
-
+    sequence, *places = torch.tensor(touched, dtype=torch.int64, device=device).t()
+    source, target = ((block_tables[sequence, at // block].long(), at % block) for at in places)
     if weight_caches is not None:
-        blocks, offsets = places(target, touched)
         for wc in weight_caches:
-            wc[blocks, :, offsets] = 0.0
+            wc[target[0], :, target[1]] = 0.0
     if not moved:
         return
-    slots = [(b * block + o).int() for b, o in (places(source, moved), places(target, moved))]
+    n = len(moved)
+    slots = [(b[:n] * block + o[:n]).int() for b, o in (source, target)]
     heads, dim = value_caches[0].shape[1:3]
-    key = torch.empty(len(moved), heads, dim, dtype=value_caches[0].dtype, device=device)
+    key = torch.empty(n, heads, dim, dtype=value_caches[0].dtype, device=device)
     value = torch.empty_like(key)
     for kc, vc in zip(key_caches, value_caches):
         cache_ops.gather_cached_kv(key, value, kc, vc, slots[0])
